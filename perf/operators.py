@@ -213,9 +213,9 @@ def prepare(case, seed):
                 return kept["t"]
             state["workspace"] = workspace
         elif case["op"] == "verify":
-            n, drafted = len(state["starts"]), 0 if state["draft_logits"] is None else len(state["draft_logits"])
+        XX
             state["accepted"], state["next"] = (torch.empty(n, dtype=torch.int32, device="cuda") for _ in range(2))
-            need = ops.verify_workspace_floats(len(state["logits"]), drafted, n, case["vocab"])
+            need = ops.verify_workspace_floats(len(state["logits"]), n, case["vocab"])
             state["workspace"] = torch.empty(need, dtype=torch.float32, device="cuda")
         else:
             state["w"] = ops.q4_pack(state.pop("codes"), state.pop("scales"), case["group"])
