@@ -213,7 +213,7 @@ def prepare(case, seed):
                 return kept["t"]
             state["workspace"] = workspace
         elif case["op"] == "verify":
-        XX
+            n = len(state["starts"])
             state["accepted"], state["next"] = (torch.empty(n, dtype=torch.int32, device="cuda") for _ in range(2))
             need = ops.verify_workspace_floats(len(state["logits"]), n, case["vocab"])
             state["workspace"] = torch.empty(need, dtype=torch.float32, device="cuda")
