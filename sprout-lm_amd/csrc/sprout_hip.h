@@ -461,4 +461,40 @@ int sp_qk_cross_prepare(void* stream, int dtype, const void* qk, int nq, int nkv
 // the outputs of the heads made by sp_qk_cross_prepare, mixed by talk (float32 [nq, nq]).  out [T, nq * dim], both `dtype`.
 int sp_head_mix(void* stream, int dtype, const void* o, const float* talk, int nq, int nkv, int dim, int width, void* out,
                 int T);
+
+// Attention of a batch whose sequences all begin with the same `prefix` keys (csrc/attention_shared.hip), in the pools' layout of
+// sp_attention: the keys before `prefix` are read once for all rows, through prefix_table (the numbers of the pages that hold them, the
+// prefix may end inside one), the keys from `prefix` up to a query's own through the sequence's row of block_tables.  Every query stands at
+// `prefix` or later.  tiles: (sequence, first query) of every tile of 16 queries of every sequence; max_ctx: the longest context; `tokens`:
+// rows of q and out; rows that belong to no sequence are left as they are.  head sizes up to 256; softcap 0: scores as they are;
+// sinks (null: none): float32 [nq], a logit per head that joins the denominator.  A row that sees no key but by weights of zero is zeros.
+int64_t sp_attention_shared_workspace_floats(int dtype, int hd, int nq, int nkv, int tokens, int n_tiles, int prefix, int max_ctx);
+int sp_attention_shared(void* stream, int dtype, const void* q, int q_stride, const void* k_pool, const void* v_pool,
+                        const int32_t* block_tables, int max_blocks, const int32_t* prefix_table, int prefix, const int32_t* q_start,
+                        const int32_t* q_len, const int32_t* ctx_len, const int32_t* tiles, int n_tiles, int max_ctx, int tokens,
+                        float* workspace, int64_t workspace_floats, void* out, int nq, int nkv, int hd, int page_size, int num_pages,
+                        float scale, float softcap, const float* sinks);
+
+// Drafted tokens tested against the target's probabilities with given uniform numbers (csrc/verify.hip has the formulas).  Sequence s has
+// rows starts[s] .. + lens[s]: tokens[start] its last sure token, tokens[start + 1 ..] its drafts; row start + j of logits [rows, vocab] (of
+// `dtype`) tests draft j, the last row follows all drafts.  uniform [rows] in [0, 1): one number a draft at the row that tests it, the last row's for the
+// next token.  temperature (null: all 0) one a sequence, 0: greedy.  draft_logits [drafted, vocab] with draft_rows [rows]: the row that the
+// token at that place was drawn from, negative: not drawn (both null: none was).  accepted[s]: drafts that hold; next[s]: the token after
+// them, -1 where a deciding row has NaN or +infinity or nothing but -infinity (a logit of -infinity alone is a token of probability 0), or
+// where lens[s] < 1 or rows are not there.
+int64_t sp_verify_workspace_floats(int rows, int sequences, int vocab);
+int sp_verify_drafts(void* stream, int dtype, const void* logits, int rows, int vocab, const int32_t* tokens, const int32_t* starts,
+                     const int32_t* lens, int sequences, const float* uniform, const float* temperature, const void* draft_logits, int drafted,
+                     const int32_t* draft_rows, int32_t* accepted, int32_t* next, void* workspace, int64_t workspace_floats);
+
+// Weights of 4 bits with a scale per `group` (32, 64 or 128) numbers of K: w[n, k] = (code - 8) * scale[n, k / group], code 0 .. 15.
+// sp_q4_quantize: codes [N, (K + 1) / 2], two a byte along K with the first in the low half, and scales [N, groups] of w [N, K]: scale =
+// max |w| / 7 rounded to scale_dtype, code = w / scale rounded to the nearest whole number.  sp_q4_pack: the same laid out for the product,
+// `words` sp_q4_words(N, K) of 32 bits, packed_scales [groups, N up to a multiple of 16].  sp_gemm_q4: out = x . w^T (+ bias) of x's dtype
+// (mode 0), or out (float32) += (mode 1); sums and scales are multiplied in float32.
+int64_t sp_q4_words(int N, int K);
+int sp_q4_quantize(void* stream, int w_dtype, const void* w, int N, int K, int group, void* codes, int scale_dtype, void* scales);
+int sp_q4_pack(void* stream, const void* codes, int scale_dtype, const void* scales, int N, int K, int group, void* words, void* packed_scales);
+int sp_gemm_q4(void* stream, int x_dtype, const void* x, const void* words, int scale_dtype, const void* scales, int bias_dtype,
+               const void* bias, int mode, int out_dtype, void* out, int T, int N, int K, int group);
 }

@@ -61,6 +61,14 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _here(what: str, *tensors) -> None:
+    """Every tensor without gaps on the current device, whose stream the launch goes to."""
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and (t.get_device() != device or device < 0 or not t.is_contiguous()):
+            raise KernelError(f"{what}: operands must be contiguous and live on the current GPU; got {tuple(t.shape)} on {t.device}.")
+
+
 # Variants of an operation that a part may ask for, as the C interface numbers them.  Only the listed ones have
 # kernels; anything else is refused (KernelError) before a launch.
 ROTARY_PAIRINGS = {"halves": 0}          # dimension d turns with d + rotary_dim / 2 ("neox"); the latent mixer's own
@@ -580,6 +588,72 @@ def gemm(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: torch.Tensor
                             _code(out, "gemm output"), out.data_ptr(), T, N, K))
 
 
+Q4_GROUPS = (32, 64, 128)      # numbers of K that share a scale
+
+
+class Q4Matrix:
+    """Weights of 4 bits as `gemm_q4` reads them: w[n, k] = (code - 8) * scale[n, k // group].  Made by `q4_pack`."""
+
+    def __init__(self, rows: int, cols: int, group: int, words: torch.Tensor, scales: torch.Tensor):
+        self.rows, self.cols, self.group, self.words, self.scales = rows, cols, group, words, scales
+
+    def nbytes(self) -> int:
+        return 4 * self.words.numel() + self.scales.element_size() * self.scales.numel()
+
+
+def _q4_sizes(N: int, K: int, group: int) -> int:
+    """Groups of a row."""
+    if group not in Q4_GROUPS or N <= 0 or K <= 0:
+        raise KernelError(f"4-bit weights [{N}, {K}] in groups of {group}: groups of {Q4_GROUPS} of a matrix that is not empty expected")
+    return -(-K // group)
+
+
+def q4_quantize(w: torch.Tensor, group: int, scale_dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of w [N, K] (float32 or bfloat16): scales [N, ceil(K / group)] = max |w| of the group / 7, rounded to `scale_dtype`;
+    codes uint8 [N, ceil(K / 2)], two a byte, the first in the low half: round(w / scale) + 8, in 0 .. 15.  A group that holds NaN or an
+    infinity has that as its scale."""
+    _here("q4_quantize", w)
+    if w.dim() != 2 or scale_dtype not in _CODES:
+        raise KernelError(f"q4_quantize: a matrix and scales in float32 or bfloat16 expected, got {tuple(w.shape)} and {scale_dtype}")
+    N, K = w.shape
+    groups = _q4_sizes(N, K, group)
+    codes = torch.empty(N, (K + 1) // 2, dtype=torch.uint8, device=w.device)
+    scales = torch.empty(N, groups, dtype=scale_dtype, device=w.device)
+    check(library().sp_q4_quantize(_stream(), _code(w, "weights"), w.data_ptr(), N, K, group, codes.data_ptr(), _CODES[scale_dtype], scales.data_ptr()))
+    return codes, scales
+
+
+def q4_pack(codes: torch.Tensor, scales: torch.Tensor, group: int, cols: int | None = None) -> Q4Matrix:
+    """Lays codes and scales (as `q4_quantize` makes them) out for `gemm_q4`; once, when a model is loaded.  `cols`: K, by default
+    twice the bytes of a row (an odd K has to be said)."""
+    _here("q4_pack", codes, scales)
+    if codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dim() != 2:
+        raise KernelError(f"q4_pack: codes uint8 [N, K / 2] and scales [N, groups] expected, got {tuple(codes.shape)} {codes.dtype} and {tuple(scales.shape)}")
+    N, K = codes.shape[0], 2 * codes.shape[1] if cols is None else int(cols)
+    groups = _q4_sizes(N, K, group)
+    if (K + 1) // 2 != codes.shape[1] or tuple(scales.shape) != (N, groups):
+        raise KernelError(f"q4_pack: [{N}, {K}] in groups of {group} has {(K + 1) // 2} bytes and {groups} scales a row; got {tuple(codes.shape)} and {tuple(scales.shape)}")
+    words = torch.empty(library().sp_q4_words(N, K), dtype=torch.int32, device=codes.device)
+    packed = torch.empty(groups, (N + 15) // 16 * 16, dtype=scales.dtype, device=codes.device)
+    check(library().sp_q4_pack(_stream(), codes.data_ptr(), _code(scales, "scales"), scales.data_ptr(), N, K, group, words.data_ptr(), packed.data_ptr()))
+    return Q4Matrix(N, K, group, words, packed)
+
+
+def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False) -> None:
+    """out = a @ w.T (+ bias) of a's dtype (float32 or bfloat16); with accumulate, out (float32) += a @ w.T (+ bias).  Made for few tokens: the
+    weights are read once for every 64 (float32: 32)."""
+    _here("gemm_q4", a, w.words, w.scales, out, bias)
+    if a.dim() != 2 or a.shape[1] != w.cols or tuple(out.shape) != (a.shape[0], w.rows):
+        raise KernelError(f"gemm_q4: shapes do not fit: a {tuple(a.shape)}, w [{w.rows}, {w.cols}], out {tuple(out.shape)}")
+    if out.dtype != (torch.float32 if accumulate else a.dtype):
+        raise KernelError(f"gemm_q4: an output of {out.dtype}; a product of {a.dtype} is stored as that or added to float32")
+    if bias is not None and bias.numel() != w.rows:
+        raise KernelError(f"gemm_q4: bias has {bias.numel()} values for {w.rows} columns")
+    check(library().sp_gemm_q4(_stream(), _code(a, "input"), a.data_ptr(), w.words.data_ptr(), _CODES[w.scales.dtype], w.scales.data_ptr(),
+                               _code(bias, "bias") if bias is not None else 0, _ptr(bias), int(accumulate), _code(out, "output"),
+                               out.data_ptr(), a.shape[0], w.rows, w.cols, w.group))
+
+
 @functools.lru_cache(maxsize=4096)
 def gemm_parts_plan(dtype: torch.dtype, T: int, N: int, K: int) -> int:
     """Parts of K in which the product of T tokens by w [N, K], both of `dtype`, is better stored (`gemm_parts`) than added to a float32
@@ -734,16 +808,17 @@ class AttentionBatch:
     """The device-side description of a step's sequences that `attention` reads."""
 
     def __init__(self, q_start, q_len, ctx_len, n_seqs: int, lists: dict, max_decode_ctx: int, max_ctx: int,
-                 mean_walk: int = 0, max_tile_ctx: int | None = None, one_query_keys: int = 0):
+                 mean_walk: int = 0, max_tile_ctx: int | None = None, one_query_keys: int = 0, first_query: int | None = None):
         """`lists`: name -> (device int32 tensor, number of entries), names as in `attention_lists`;
         `max_decode_ctx`, `max_ctx`: the longest context among one-query sequences, and among all;
         `mean_walk`: the mean number of keys that a tile of queries walks, see `mean_tile_walk` (a hint for
         how the kernels share out the work; unknown: 0); `max_tile_ctx`: the longest context among sequences with several
         queries (a hint as well; by default the longest of all); `one_query_keys`: the sum of the one-query sequences'
-        contexts (a hint as well; unknown: 0)."""
+        contexts (a hint as well; unknown: 0); `first_query`: the lowest position that any query stands at (None: unknown;
+        `attention_shared` asks for it)."""
         self.q_start, self.q_len, self.ctx_len, self.n_seqs = q_start, q_len, ctx_len, n_seqs
         self.lists, self.max_decode_ctx, self.max_ctx = lists, max_decode_ctx, max_ctx
-        self.mean_walk, self.one_query_keys = mean_walk, one_query_keys
+        self.mean_walk, self.one_query_keys, self.first_query = mean_walk, one_query_keys, first_query
         self.max_tile_ctx = max_ctx if max_tile_ctx is None else max_tile_ctx
 
     @classmethod
@@ -757,7 +832,7 @@ class AttentionBatch:
         return cls(to(starts), to(q_lens), to(ctx_lens), len(q_lens), lists, max(decode_ctx, default=0),
                    max((int(c) for c in ctx_lens), default=0),
                    mean_tile_walk(q_lens, ctx_lens), max((int(c) for c, q in zip(ctx_lens, q_lens) if q > 1), default=0),
-                   sum(int(c) for c in decode_ctx))
+                   sum(int(c) for c in decode_ctx), min((int(c) - int(q) for c, q in zip(ctx_lens, q_lens) if q > 0), default=None))
 
 
 def attention_plan(dtype: torch.dtype, hd: int, page_size: int, nq: int, nkv: int, kind: int = 0) -> tuple[int, bool]:
@@ -885,6 +960,73 @@ def attention(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_pool: torc
                                  need, out.data_ptr(), nq, nkv, hd, page_size, num_pages, int(window) if window else 0,
                                  float(scale), kind, scores_code, *stage, keep_first, _ptr(weight_bias), gate_ptr, gate_stride))
     return False
+
+
+MAX_SHARED_HEAD_DIM = 256      # the largest head size that attention_shared takes
+
+
+def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
+                     batch: AttentionBatch, prefix: int, out: torch.Tensor, nq: int, nkv: int, hd: int, scale: float, workspace=None,
+                     scores: str = "scaled_dot", softcap: float = 0.0, sinks: torch.Tensor | None = None,
+                     prefix_table: torch.Tensor | None = None) -> None:
+    """Causal attention, as `attention` without a window, of a batch whose sequences all begin with the same `prefix` tokens: their keys
+    and values are read once for all rows, and each sequence's own keys, from position `prefix` on, by its own queries.
+
+    Every query stands at position `prefix` or later (`batch.first_query` says so; a call that does not is refused).  The shared keys are
+    read through `prefix_table` (int32, the pages of tokens 0 .. prefix - 1), by default the first sequence's row of `block_tables`; a
+    prefix that ends inside a page may have a copy of its end in each sequence's own page.  Any number of queries a sequence, any page
+    size, head sizes up to 256.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new one); calls
+    that may run at the same time need one each.  `scores`, `softcap`, `sinks`: as for `attention`.  Rows of `out` that belong
+    to no sequence are left as they are."""
+    code = _code(q, "q")
+    if variant_code(SCORE_STAGES, scores, "score stage") == 1:
+        if not softcap > 0.0:
+            raise KernelError("attention_shared: capped scores need a positive cap")
+    else:
+        softcap = 0.0
+    if nkv <= 0 or nq <= 0 or nq % nkv or not 0 < hd <= MAX_SHARED_HEAD_DIM:
+        raise KernelError(f"attention_shared: {nq} query heads of {hd} in {nkv} groups: heads of 1..{MAX_SHARED_HEAD_DIM} that divide into the groups expected")
+    tiles, n_tiles = batch.lists["tiles_all_16"]
+    _here("attention_shared", q, k_pool, v_pool, block_tables, out, sinks, prefix_table, batch.q_start, batch.q_len, batch.ctx_len,
+          tiles if n_tiles else None)
+    if q.dim() != 2 or out.dim() != 2 or out.shape[1] != nq * hd or q.shape[0] < out.shape[0] or q.dtype != out.dtype \
+            or not nq * hd <= q_stride <= q.shape[1]:
+        raise KernelError(f"attention_shared: shapes or dtypes do not fit: q {tuple(q.shape)} {q.dtype}, row stride {q_stride}, out {tuple(out.shape)} {out.dtype}")
+    if q_stride != q.shape[1]:
+        raise KernelError(f"attention_shared: rows of q are {q.shape[1]} numbers apart, not {q_stride}")
+    num_pages, page_size = _check_pools(k_pool, v_pool, nkv, hd, q.dtype, "attention_shared")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != nq):
+        raise KernelError(f"attention_shared: sinks must be {nq} float32 values")
+    if n_tiles == 0:
+        return
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < batch.n_seqs:
+        raise KernelError("attention_shared: block tables must be int32 [sequences, max_blocks]")
+    for t, n, what in ((batch.q_start, batch.n_seqs, "q_start"), (batch.q_len, batch.n_seqs, "q_len"), (batch.ctx_len, batch.n_seqs, "ctx_len"),
+                       (tiles, 2 * n_tiles, "tiles")):
+        if t.dtype != torch.int32 or t.numel() < n:
+            raise KernelError(f"attention_shared: {what} must be {n} int32 values")
+    max_ctx = int(batch.max_ctx)
+    if prefix < 0 or batch.first_query is None or batch.first_query < prefix:
+        raise KernelError(f"attention_shared: a query at position {batch.first_query} does not stand behind a prefix of {prefix} tokens")
+    if max_ctx > block_tables.shape[1] * page_size:
+        raise KernelError(f"attention_shared: a context of {max_ctx} tokens is longer than its block table ({block_tables.shape[1]} pages of {page_size})")
+    if prefix_table is None:
+        prefix_table = block_tables      # the first row of it
+    elif prefix_table.dtype != torch.int32 or prefix_table.numel() * page_size < prefix:
+        raise KernelError(f"attention_shared: a prefix of {prefix} tokens is longer than its table ({prefix_table.numel()} pages of {page_size})")
+    T = out.shape[0]
+    if n_tiles > T:
+        raise KernelError(f"attention_shared: {n_tiles} tiles of queries for {T} rows")
+    lib = library()
+    need = lib.sp_attention_shared_workspace_floats(code, hd, nq, nkv, T, n_tiles, prefix, max_ctx)
+    ws = workspace(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
+    _here("attention_shared", ws)
+    if ws.dtype != torch.float32 or ws.numel() < need or ws.data_ptr() % 16:
+        raise KernelError(f"attention_shared: the workspace must hold {need} float32 values at a multiple of 16 bytes")
+    check(lib.sp_attention_shared(_stream(), code, q.data_ptr(), q_stride, k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
+                                  block_tables.shape[1], prefix_table.data_ptr(), prefix, batch.q_start.data_ptr(), batch.q_len.data_ptr(),
+                                  batch.ctx_len.data_ptr(), tiles.data_ptr(), n_tiles, max_ctx, T, ws.data_ptr(), need, out.data_ptr(), nq, nkv,
+                                  hd, page_size, num_pages, float(scale), float(softcap), _ptr(sinks)))
 
 
 def feed_tokens(tokens: torch.Tensor, previous: torch.Tensor, source: torch.Tensor, vocab: int) -> None:
@@ -1526,6 +1668,51 @@ def sample(logits: torch.Tensor, out: torch.Tensor, workspace: torch.Tensor, tem
             raise KernelError("sample: temperature must be float32 and seed int64, one per row")
     check(library().sp_sample(_stream(), logits.data_ptr(), _ptr(temperature), _ptr(seed), _ptr(counter), out.data_ptr(),
                               workspace.data_ptr(), R, V))
+
+
+def verify_workspace_floats(rows: int, sequences: int, vocab: int) -> int:
+    """float32 values of workspace that `verify_drafts` wants."""
+    return library().sp_verify_workspace_floats(rows, sequences, vocab)
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, uniform: torch.Tensor | None,
+                  accepted: torch.Tensor, next_token: torch.Tensor, workspace: torch.Tensor, temperature: torch.Tensor | None = None,
+                  draft_logits: torch.Tensor | None = None, draft_rows: torch.Tensor | None = None) -> None:
+    """Tests drafted tokens against the target's probabilities and draws the token after those that hold.
+
+    Sequence s has rows starts[s] .. + lens[s] of `logits` (float32 or bfloat16 [rows, vocab], the logits of a step at every token of the
+    sequence) and of `tokens` (int32, that step's token ids: the last sure one, then the drafts).  With p = softmax(logits[r] / temperature)
+    and q the same of `draft_logits[draft_rows[r + 1]]`, the row that tokens[r + 1] was drawn from (a negative row, or none of these: q is 1
+    at the draft), the draft holds while uniform[r] q(draft) < p(draft).  `accepted[s]`: how many drafts hold; `next_token[s]`: drawn from
+    max(p - q, 0) of the first that does not, from p of the last row where all do, as the lowest index whose running sum exceeds
+    uniform[last row] times the whole; so the tokens are distributed as p has them.  Where the temperature is 0 (or absent) a draft
+    holds while it is the lowest index of the maximum, and the next token is that index.  A logit of -infinity is a token that is not
+    allowed; a deciding row with NaN or +infinity, or without any token allowed, gives next_token -1, as `sample` does.
+    starts, lens: int32, one a sequence; uniform: float32 in [0, 1), one a row; temperature: float32, one a sequence; accepted, next_token: int32."""
+    _here("verify_drafts", logits, tokens, starts, lens, uniform, accepted, next_token, workspace, temperature, draft_logits, draft_rows)
+    code = _code(logits, "logits")
+    if logits.dim() != 2:
+        raise KernelError(f"verify_drafts: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
+    R, V = logits.shape
+    n = starts.numel()
+    for t, count, what in ((tokens, R, "tokens"), (starts, n, "starts"), (lens, n, "lens"), (accepted, n, "accepted"), (next_token, n, "next tokens"),
+                           (draft_rows, R, "draft rows")):
+        if t is not None and (t.dtype != torch.int32 or t.numel() < count):
+            raise KernelError(f"verify_drafts: {what} must be {count} int32 values, got {t.numel()} of {t.dtype}")
+    for t, count, what in ((uniform, R, "uniform numbers"), (temperature, n, "temperatures")):
+        if t is not None and (t.dtype != torch.float32 or t.numel() < count):
+            raise KernelError(f"verify_drafts: {what} must be {count} float32 values, got {t.numel()} of {t.dtype}")
+    if temperature is not None and uniform is None:
+        raise KernelError("verify_drafts: sampling needs uniform numbers")
+    if (draft_logits is None) != (draft_rows is None):
+        raise KernelError("verify_drafts: draft logits and the rows of the drafts go together")
+    if draft_logits is not None and (draft_logits.dtype != logits.dtype or draft_logits.dim() != 2 or draft_logits.shape[1] != V):
+        raise KernelError(f"verify_drafts: draft logits {tuple(draft_logits.shape)} {draft_logits.dtype} do not fit logits {tuple(logits.shape)} {logits.dtype}")
+    if workspace.dtype != torch.float32:
+        raise KernelError("verify_drafts: the workspace must be float32")
+    check(library().sp_verify_drafts(_stream(), code, logits.data_ptr(), R, V, tokens.data_ptr(), starts.data_ptr(), lens.data_ptr(), n,
+                                     _ptr(uniform), _ptr(temperature), _ptr(draft_logits), 0 if draft_logits is None else draft_logits.shape[0],
+                                     _ptr(draft_rows), accepted.data_ptr(), next_token.data_ptr(), workspace.data_ptr(), workspace.numel()))
 
 
 def probe_machine(device=None, megabytes: int = 4096, repeats: int = 5) -> dict:
