@@ -8,10 +8,13 @@
 // Temperature 0: draft j holds while it is the lowest index of the row's maximum, which is the next token.
 //
 // The answers are whole numbers, and a running sum over 150,000 tokens passes as many borders: exponentials and sums are float64, whose
-// vector rate equals float32's here, so that the sum's order moves an answer about once in 10^11 draws (float32: once in a thousand).
+// vector rate equals float32's here, so that their errors (2e-13 of a weight) move an answer once in some 10^7 draws; float32 sums would
+// once in a thousand.  The exponential is 2^n times the Taylor polynomial of 2^f, |f| <= 1/2, of degree 10: 17 instructions a logit, with which
+// reading the rows still takes longer than weighing them (the library's exponential took 184 us for 646 rows of 152,064, this 75).
 //
-// Three launches: maximum and sum of every row by chunks, so that few rows fill the chip as many do; then a block per chunk and sequence
-// joins the chunks' statistics, finds the deciding row and sums its chunk of what is left; then a block per sequence finds chunk and token.
+// Four launches: maximum and sum of every row by chunks, so that few rows fill the chip as many do; a block per sequence, a wave a row,
+// joins them and finds the deciding row; a block per chunk and sequence sums what is left there; a block per sequence finds chunk and token.
+// (The second and third in one, every block of a sequence deciding by itself: 52 us of 64 sequences, where these take DECIDE and LEFT.)
 #include "common.h"
 #include "sprout_hip.h"
 
@@ -21,9 +24,9 @@ namespace {
 
 constexpr int kVerifyChunk = 4096;      // logits of a block: 16 a thread
 
-struct ChunkStat { double sum; float top; int32_t best; };                   // sum of exp((l - top) / temperature); best: index of top, -1: no good row
+struct ChunkStat { double sum; float top; int32_t best; };      // sum of exp((l - top) / temperature), or (greedy) the lowest index of top; best -1: NaN or +infinity
 struct RowStat { double sum; float top; int32_t best; };
-struct Decision { double p_scale, q_scale; float p_top, q_top; int32_t row, draft_row, draft, kind; };   // kind: 0 from p, 1 from what is left, 2 settled
+struct Decision { double p_scale, q_scale, degree, u; float p_top, q_top; int32_t row, draft_row, draft, kind; };      // kind: 0 from p, 1 from what is left, 2 settled; u: the last uniform number
 
 struct VerifyArgs {
   const void *logits, *draft_logits;
@@ -44,19 +47,81 @@ __device__ __forceinline__ double wave_sum64(double v) {
 __device__ __forceinline__ void better(float& v, int& i, float ov, int oi) {
   if (ov > v || (ov == v && oi < i)) { v = ov; i = oi; }
 }
-__device__ __forceinline__ double weight(float l, float top, double per_degree) {
-  return l == -INFINITY ? 0.0 : exp((double(l) - double(top)) * per_degree);
+// 2^y for y <= 0, 0 where that has no float64 (a token that is not allowed weighs nothing): 2^n times the Taylor polynomial of 2^f, whose
+// coefficients are ln(2)^k / k!, of degree 8 (2e-10 of the value).  y + 1.5 * 2^52 leaves n in the low word of the sum.
+__device__ __forceinline__ double two_to(double y) {
+  y = fmax(y, -1100.0);
+  const double shifted = y + 6755399441055744.0, f = y - (shifted - 6755399441055744.0);
+  const int n = int(__double_as_longlong(shifted));
+  double p = 1.3215486790144310e-06;
+  p = fma(p, f, 1.5252733804059840e-05);
+  p = fma(p, f, 1.5403530393381610e-04);
+  p = fma(p, f, 1.3333558146428443e-03);
+  p = fma(p, f, 9.6181291076284772e-03);
+  p = fma(p, f, 5.5504108664821580e-02);
+  p = fma(p, f, 2.4022650695910072e-01);
+  p = fma(p, f, 6.9314718055994531e-01);
+  p = fma(p, f, 1.0);
+  return ldexp(p, n);
 }
+// The same for the sums over whole rows, to 1e-9 of the value, with six float64 instructions (they take twice a float32's time) for sixteen:
+// y with 32 bits behind the point is the low word of y + 1.5 * 2^20 and n the bits above it; 2^f is a table's 2^(k / 64) times 1 + a
+// cubic in what is left, at most 0.011, which float32 holds to 1e-9.  2^-1000 below that, which no sum notices.
+__device__ __forceinline__ double table_power(const double* table, double diff, double degree) {
+  const long long bits = __double_as_longlong(fmax(diff * degree, -1000.0) + 1572864.0);
+  const uint32_t low = uint32_t(bits);
+  const float r = float(low & 0x03ffffffu) * 0x1p-32f;
+  const double t = table[low >> 26];
+  const float q = r * fmaf(r, fmaf(r, 5.5504109e-02f, 2.4022651e-01f), 6.9314718e-01f);
+  const long long power = __double_as_longlong(fma(t, double(q), t));
+  return __longlong_as_double((long long)(uint32_t(power >> 32) + (uint32_t(bits >> 32) << 20)) << 32 | uint32_t(power));
+}
+// Temperatures are handled as `degree` = log2(e) / temperature: a logit weighs 2^((l - top) degree).  (The difference first: a product of
+// the largest logits rounds by more than any difference.)
+__device__ __forceinline__ double degree_of(float temperature) { return 1.4426950408889634 / double(temperature); }
+__device__ __forceinline__ double weight(float l, double top, double degree) { return two_to((double(l) - top) * degree); }
 __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int s) { return a.temperature ? a.temperature[s] : 0.f; }
 
-template <typename T>
+// Sixteen logits of a chunk to a thread: groups of four, 1,024 apart (VEC), or single ones 256 apart.  What lies behind the row is -infinity.
+template <typename T, bool VEC> __device__ __forceinline__ int logit_index(int chunk, int j) {
+  return chunk * kVerifyChunk + (VEC ? 4 * int(threadIdx.x) + 1024 * (j / 4) + j % 4 : int(threadIdx.x) + 256 * j);
+}
+__device__ __forceinline__ void load_four(const float* row, int i, int vocab, float* v) {      // (vocab is whole fours)
+  const float4 x = i < vocab ? *reinterpret_cast<const float4*>(row + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+__device__ __forceinline__ void load_four(const bf16_t* row, int i, int vocab, float* v) {
+  const uint2 x = i < vocab ? *reinterpret_cast<const uint2*>(row + i) : make_uint2(0xff80ff80u, 0xff80ff80u);
+  v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
+  v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
+}
+template <typename T, bool VEC> __device__ __forceinline__ void load_logits(const T* row, int chunk, int vocab, float (&v)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; j += VEC ? 4 : 1) {
+    const int i = logit_index<T, VEC>(chunk, j);
+    if (VEC) load_four(row, i, vocab, v + j);
+    else v[j] = i < vocab ? to_float(row[i]) : -INFINITY;
+  }
+}
+
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
+  __shared__ double s_powers[64];
   __shared__ float s_top[4];
-  __shared__ int s_best[4], s_seq, s_bad;
+  __shared__ int s_best, s_seq;
   __shared__ double s_sum[4];
-  const int chunk = blockIdx.x, place = blockIdx.y % a.rows;
+  const int chunk = blockIdx.x, place = int(blockIdx.y) >= a.rows ? blockIdx.y - a.rows : blockIdx.y;
   const bool drafter = int(blockIdx.y) >= a.rows;
-  if (threadIdx.x == 0) { s_seq = -1; s_bad = 0; }
+  int row = place;
+  if (drafter) {
+    row = a.draft_rows[place];
+    if (row < 0 || row >= a.drafted) return;
+  }
+  // the row is asked for before it is known whose it is
+  float v[16];
+  load_logits<T, VEC>(static_cast<const T*>(drafter ? a.draft_logits : a.logits) + size_t(row) * a.vocab, chunk, a.vocab, v);
+  if (threadIdx.x < 64) s_powers[threadIdx.x] = two_to(double(threadIdx.x) / 64.0 - 1.0) * 2.0;
+  if (threadIdx.x == 0) { s_seq = -1; s_best = 0x7fffffff; }
   __syncthreads();
   for (int s = threadIdx.x; s < a.sequences; s += 256) {
     const int at = place - a.starts[s];
@@ -66,144 +131,175 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   const int seq = s_seq;
   if (seq < 0) return;
   const float temp = temperature_of(a, seq);
-  int row = place;
-  if (drafter) {
-    row = a.draft_rows[place];
-    if (!(temp > 0.f) || row < 0 || row >= a.drafted) return;
-  }
-  const T* src = static_cast<const T*>(drafter ? a.draft_logits : a.logits) + size_t(row) * a.vocab;
-  const int begin = chunk * kVerifyChunk;
-  float v[16], top = -INFINITY;
-  int best = 0x7fffffff;
-  bool bad = false;
+  if (drafter && !(temp > 0.f)) return;
+  const bool greedy = !(temp > 0.f);
+  // the maximum that is NaN where a number is: NaN and +infinity make a row that is not taken
+  float top = v[0];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int i = begin + threadIdx.x + 256 * j;
-    v[j] = i < a.vocab ? to_float(src[i]) : -INFINITY;
-    bad |= !(v[j] < INFINITY);      // NaN or +infinity; a token whose logit is -infinity has probability 0
-    if (i < a.vocab) better(top, best, v[j], i);
-  }
+  for (int j = 1; j < 16; ++j) top = __builtin_elementwise_maximum(top, v[j]);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) better(top, best, __shfl_xor(top, o, 64), __shfl_xor(best, o, 64));
+  for (int o = 32; o > 0; o >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o, 64));
   const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) { s_top[wave] = top; s_best[wave] = best; }
-  if (bad) s_bad = 1;
+  if ((threadIdx.x & 63) == 0) s_top[wave] = top;
   __syncthreads();
-  for (int w = 0; w < 4; ++w) better(top, best, s_top[w], s_best[w]);
+  for (int w = 0; w < 4; ++w) top = __builtin_elementwise_maximum(top, s_top[w]);
+  const bool good = top < INFINITY;
+  int best = 0x7fffffff;
   double sum = 0.0;
-  if (temp > 0.f && top > -INFINITY) {
-    const double per_degree = 1.0 / double(temp);
+  if (greedy) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum += weight(v[j], top, per_degree);
+    for (int j = 15; j >= 0; --j) {
+      const int i = logit_index<T, VEC>(chunk, j);
+      if (i < a.vocab && v[j] == top) best = min(best, i);
+    }
+    if (best != 0x7fffffff) atomicMin(&s_best, best);
+  } else if (good && top > -INFINITY) {
+    const double degree = degree_of(temp), from = double(top);
+    double sums[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sums[j % 4] += table_power(s_powers, double(v[j]) - from, degree);
+    sum = wave_sum64((sums[0] + sums[1]) + (sums[2] + sums[3]));
+    if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
   }
-  sum = wave_sum64(sum);
-  if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0)
-    a.stats[(size_t(blockIdx.y)) * a.chunks + chunk] = {s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], top, s_bad ? -1 : best};
+    a.stats[(size_t(blockIdx.y)) * a.chunks + chunk] = {greedy || !(top > -INFINITY) || !good ? 0.0 : s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], top,
+                                                        !good ? -1 : greedy ? s_best : 0};
 }
 
 // A wave: the statistics of one row from its chunks'.  best -1: NaN, +infinity, or nothing but -infinity.
-__device__ __forceinline__ RowStat row_stat(const ChunkStat* stats, int chunks, double per_degree) {
+__device__ __forceinline__ RowStat row_stat(const ChunkStat* stats, int chunks, double degree) {
   const int lane = threadIdx.x & 63;
   float top = -INFINITY;
   int best = 0x7fffffff, bad = 0;
+  const ChunkStat first = lane < chunks ? stats[lane] : ChunkStat{0.0, -INFINITY, 0x7fffffff};
   for (int c = lane; c < chunks; c += 64) {
-    const ChunkStat st = stats[c];
+    const ChunkStat st = c == lane ? first : stats[c];
     if (st.best < 0) bad = 1;
     better(top, best, st.top, st.best);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    better(top, best, __shfl_xor(top, o, 64), __shfl_xor(best, o, 64));
+    const float ov = __shfl_xor(top, o, 64);
+    const int oi = __shfl_xor(best, o, 64);
+    better(top, best, ov, oi);
     bad |= __shfl_xor(bad, o, 64);
   }
   double sum = 0.0;
-  for (int c = lane; c < chunks; c += 64) sum += stats[c].sum * weight(stats[c].top, top, per_degree);
+  for (int c = lane; c < chunks; c += 64) {
+    const ChunkStat st = c == lane ? first : stats[c];
+    if (st.top > -INFINITY) sum += st.sum * weight(st.top, double(top), degree);
+  }
   return {wave_sum64(sum), top, bad || !(top > -INFINITY) ? -1 : best};
 }
 
-// What is left of token i's probability in the deciding row.
-template <typename T> __device__ __forceinline__ double left_of(const Decision& d, const T* row, const T* draft_row, int i, double per_degree) {
-  const double p = weight(to_float(row[i]), d.p_top, per_degree) * d.p_scale;
-  if (d.kind == 0) return p;
-  const double q = draft_row ? weight(to_float(draft_row[i]), d.q_top, per_degree) * d.q_scale : i == d.draft ? 1.0 : 0.0;
-  return p > q ? p - q : 0.0;
-}
-
 template <typename T>
-__global__ __launch_bounds__(256) void verify_decide_kernel(VerifyArgs a) {
-  __shared__ Decision s_found[4];
-  __shared__ int s_holds[4], s_next[4];
-  __shared__ double s_sum[4];
-  const int chunk = blockIdx.x, seq = blockIdx.y, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(512) void verify_decide_kernel(VerifyArgs a) {
+  constexpr int kRows = 8;      // rows of a sequence at a time, a wave each; the last row of a sequence never holds
+  __shared__ Decision s_found[kRows];
+  __shared__ int s_holds[kRows], s_next[kRows];
+  const int seq = blockIdx.x, wave = threadIdx.x >> 6;
   const int start = a.starts[seq], len = a.lens[seq];
   if (len <= 0 || start < 0 || start > a.rows - len) {      // rows that are not there
-    if (chunk == 0 && threadIdx.x == 0) { a.accepted[seq] = 0; a.next[seq] = -1; a.decisions[seq].kind = 2; }
+    if (threadIdx.x == 0) { a.accepted[seq] = 0; a.next[seq] = -1; a.decisions[seq].kind = 2; }
     return;
   }
   const float temp = temperature_of(a, seq);
   const bool greedy = !(temp > 0.f);
-  const double per_degree = greedy ? 0.0 : 1.0 / double(temp);
-  int accepted = -1;
-  Decision d;
-  int next = -1;
-  for (int first = 0; accepted < 0; first += 4) {      // four drafts at a time; the last row of a sequence never holds
+  const double degree = greedy ? 0.0 : degree_of(temp), last_u = greedy ? 0.0 : double(a.uniform[start + len - 1]);
+  for (int first = 0;; first += kRows) {
     const int j = first + wave;
     if (j < len) {
       const int place = start + j;
-      const RowStat p = row_stat(a.stats + size_t(place) * a.chunks, a.chunks, per_degree);
-      Decision mine = {1.0 / p.sum, 0.0, p.top, 0.f, place, -1, -1, 0};
+      const bool tested = j < len - 1;
+      const int draft = tested ? a.tokens[place + 1] : -1, from = tested && a.draft_rows && !greedy ? a.draft_rows[place + 1] : -1;
+      const bool known = draft >= 0 && draft < a.vocab, drawn = from >= 0 && from < a.drafted;
+      // all that the row needs is asked for together
+      const float l_p = known ? to_float(static_cast<const T*>(a.logits)[size_t(place) * a.vocab + draft]) : 0.f;
+      const float l_q = known && drawn ? to_float(static_cast<const T*>(a.draft_logits)[size_t(from) * a.vocab + draft]) : 0.f;
+      const float u = tested && !greedy ? a.uniform[place] : 0.f;
+      RowStat q = {1.0, 0.f, -1};
+      if (drawn) q = row_stat(a.stats + (size_t(a.rows) + place + 1) * a.chunks, a.chunks, degree);
+      const RowStat p = row_stat(a.stats + size_t(place) * a.chunks, a.chunks, degree);
+      Decision mine = {1.0 / p.sum, 0.0, degree, last_u, p.top, 0.f, place, -1, -1, tested ? 1 : 0};
       bool holds = false;
       int token = p.best;      // what is next where the row settles that without a draw: the greedy choice, or -1
-      if (p.best < 0) {
+      if (p.best < 0 || greedy) {
         mine.kind = 2;
-      } else if (greedy) {
-        mine.kind = 2;
-        holds = j < len - 1 && a.tokens[place + 1] == p.best;
-      } else if (j < len - 1) {
-        const int draft = a.tokens[place + 1];
-        const int from = a.draft_rows ? a.draft_rows[place + 1] : -1;
-        const bool known = draft >= 0 && draft < a.vocab;
-        double q_draft = 1.0;
-        mine.kind = 1;
+        holds = p.best >= 0 && tested && draft == p.best;
+      } else if (tested) {
         mine.draft = draft;
+        double q_draft = 1.0;
         if (from >= 0) {
           mine.draft_row = from;
-          const RowStat q = from < a.drafted ? row_stat(a.stats + (size_t(a.rows) + place + 1) * a.chunks, a.chunks, per_degree)
-                                             : RowStat{1.0, 0.f, -1};
+          mine.q_scale = 1.0 / q.sum;
+          mine.q_top = q.top;
           if (q.best < 0) { mine.kind = 2; token = -1; }
-          else {
-            mine.q_scale = 1.0 / q.sum;
-            mine.q_top = q.top;
-            q_draft = known ? weight(to_float(static_cast<const T*>(a.draft_logits)[size_t(from) * a.vocab + draft]), q.top, per_degree) * mine.q_scale : 0.0;
-          }
+          else q_draft = weight(l_q, double(q.top), degree) * mine.q_scale;
         }
-        if (mine.kind == 1 && known) {
-          const double p_draft = weight(to_float(static_cast<const T*>(a.logits)[size_t(place) * a.vocab + draft]), p.top, per_degree) * mine.p_scale;
-          holds = double(a.uniform[place]) * q_draft < p_draft;
-        }
+        holds = mine.kind == 1 && known && double(u) * q_draft < weight(l_p, double(p.top), degree) * mine.p_scale;
       }
       if ((threadIdx.x & 63) == 0) { s_found[wave] = mine; s_holds[wave] = holds; s_next[wave] = token; }
     }
     __syncthreads();
-    for (int w = 0; w < 4 && accepted < 0; ++w)
-      if (first + w < len && !s_holds[w]) { accepted = first + w; d = s_found[w]; next = s_next[w]; }
+    const int n = min(kRows, len - first);
+    int stop = 0;
+    while (stop < n && s_holds[stop]) ++stop;
+    if (stop < n) {      // (the same in every thread)
+      if (threadIdx.x == 0) {
+        a.accepted[seq] = first + stop;
+        a.decisions[seq] = s_found[stop];
+        if (s_found[stop].kind == 2) a.next[seq] = s_next[stop];
+      }
+      return;
+    }
     __syncthreads();
   }
-  if (chunk == 0 && threadIdx.x == 0) {
-    a.accepted[seq] = accepted;
-    a.decisions[seq] = d;
-    if (d.kind == 2) a.next[seq] = next;
-  }
+}
+
+// What is left of a token's probability in the deciding row, of logits p and q (drawn: q from the drafter's row).  kind 0: all of it, else
+// what p has more than q.
+__device__ __forceinline__ double left_of(const Decision& d, bool drawn, double degree, float p, float q, int token) {
+  const double mine = weight(p, double(d.p_top), degree) * d.p_scale;
+  if (d.kind == 0) return mine;
+  const double other = drawn ? weight(q, double(d.q_top), degree) * d.q_scale : token == d.draft ? 1.0 : 0.0;
+  return mine > other ? mine - other : 0.0;
+}
+
+// (Loops that are not unrolled over the sixteen: few blocks run these, and code that is run once costs its own way from memory.)
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void verify_left_kernel(VerifyArgs a) {
+  __shared__ double s_sum[4];
+  const int chunk = blockIdx.x, seq = blockIdx.y, wave = threadIdx.x >> 6;
+  const Decision d = a.decisions[seq];
   if (d.kind == 2) return;
+  const bool drawn = d.kind == 1 && d.draft_row >= 0;
   const T* row = static_cast<const T*>(a.logits) + size_t(d.row) * a.vocab;
-  const T* draft_row = d.draft_row >= 0 ? static_cast<const T*>(a.draft_logits) + size_t(d.draft_row) * a.vocab : nullptr;
-  double sum = 0.0;
+  const T* draft_row = drawn ? static_cast<const T*>(a.draft_logits) + size_t(d.draft_row) * a.vocab : row;
+  const double degree = d.degree;
+  float p[4], q[4];
+  auto load = [&](int group) __attribute__((always_inline)) {
+    const int i = chunk * kVerifyChunk + 1024 * group + (VEC ? 4 : 1) * int(threadIdx.x);
+    if (VEC) {
+      load_four(row, i, a.vocab, p);
+      load_four(draft_row, i, a.vocab, q);
+    } else {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int i = chunk * kVerifyChunk + threadIdx.x + 256 * j;
-    if (i < a.vocab) sum += left_of(d, row, draft_row, i, per_degree);
+      for (int j = 0; j < 4; ++j) {
+        p[j] = i + 256 * j < a.vocab ? to_float(row[i + 256 * j]) : -INFINITY;
+        q[j] = i + 256 * j < a.vocab ? to_float(draft_row[i + 256 * j]) : -INFINITY;
+      }
+    }
+  };
+  double sum = 0.0;
+  load(0);
+#pragma unroll 1
+  for (int group = 0; group < 4; ++group) {
+    const float p_now[4] = {p[0], p[1], p[2], p[3]}, q_now[4] = {q[0], q[1], q[2], q[3]};
+    if (group < 3) load(group + 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      sum += left_of(d, drawn, degree, p_now[j], q_now[j], chunk * kVerifyChunk + 1024 * group + (VEC ? 4 * int(threadIdx.x) + j : int(threadIdx.x) + 256 * j));
   }
   sum = wave_sum64(sum);
   if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
@@ -211,79 +307,125 @@ __global__ __launch_bounds__(256) void verify_decide_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) a.left[size_t(seq) * a.chunks + chunk] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ double s_scan[256], s_before, s_limit;
+constexpr int kDrawThreads = kVerifyChunk / 4;
+// The sum of v over the threads before this one; `total`: over all.
+__device__ __forceinline__ double sum_before(double v, double* scratch, double& total) {
+  constexpr int WAVES = kDrawThreads / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double running = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double add = __shfl_up(running, o, 64);
+    if (lane >= o) running += add;
+  }
+  __syncthreads();      // what lay in `scratch` has been used
+  if (lane == 63) scratch[wave] = running;
+  __syncthreads();
+  double before = __shfl_up(running, 1, 64), waves = lane < WAVES ? scratch[lane] : 0.0;
+  if (lane == 0) before = 0.0;
+#pragma unroll
+  for (int o = 1; o < WAVES; o <<= 1) {
+    const double add = __shfl_up(waves, o, 64);
+    if (lane >= o) waves += add;
+  }
+  total = __shfl(waves, WAVES - 1, 64);
+  const double of_waves = __shfl(waves, wave - 1 & 63, 64);
+  return wave ? before + of_waves : before;
+}
+
+// A block per sequence, a thread a chunk and then four tokens of the chunk that the limit lies in.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ double s_scratch[kDrawThreads / 64], s_before;
   __shared__ int s_chunk, s_token, s_last;
-  const int seq = blockIdx.x;
+  const int seq = blockIdx.x, t = threadIdx.x;
   Decision d = a.decisions[seq];
   if (d.kind == 2) return;
-  const double per_degree = 1.0 / double(temperature_of(a, seq));
-  const double u = double(a.uniform[a.starts[seq] + a.lens[seq] - 1]);
-  const ChunkStat* stats = a.stats + size_t(d.row) * a.chunks;
-  if (threadIdx.x == 0) {
-    double total = 0.0;
-    for (int c = 0; c < a.chunks; ++c) total += a.left[size_t(seq) * a.chunks + c];
-    // nothing is left of p - q (a draft that neither side allows, under equal rows): the next token comes from p
-    const bool from_p = d.kind == 1 && !(total > 0.0);
-    auto mass = [&](int c) { return from_p ? stats[c].sum * weight(stats[c].top, d.p_top, per_degree) * d.p_scale : a.left[size_t(seq) * a.chunks + c]; };
-    if (from_p) {
-      total = 0.0;
-      for (int c = 0; c < a.chunks; ++c) total += mass(c);
-    }
-    const double limit = u * total;
-    double before = 0.0, running = 0.0;
-    int chunk = -1;
-    for (int c = 0; c < a.chunks; ++c) {
-      const double m = mass(c);
-      if (m > 0.0) {
-        chunk = c;
-        before = running;
-        running += m;
-        if (running > limit) break;
-      }
-    }
-    s_chunk = chunk; s_before = before; s_limit = limit;
-    s_token = from_p ? -2 : 0x7fffffff;
-    s_last = -1;
-  }
-  __syncthreads();
-  if (s_token == -2) d.kind = 0;
-  __syncthreads();
-  if (threadIdx.x == 0) s_token = 0x7fffffff;
-  const T* row = static_cast<const T*>(a.logits) + size_t(d.row) * a.vocab;
-  const T* draft_row = d.kind == 1 && d.draft_row >= 0 ? static_cast<const T*>(a.draft_logits) + size_t(d.draft_row) * a.vocab : nullptr;
-  // sixteen tokens in a row to a thread
-  double w[16], sum = 0.0;
-  const int begin = s_chunk * kVerifyChunk + 16 * threadIdx.x;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    w[j] = begin + j < a.vocab ? left_of(d, row, draft_row, begin + j, per_degree) : 0.0;
-    sum += w[j];
-  }
-  s_scan[threadIdx.x] = sum;
-  __syncthreads();
-  for (int o = 1; o < 256; o <<= 1) {
-    const double add = int(threadIdx.x) >= o ? s_scan[threadIdx.x - o] : 0.0;
-    __syncthreads();
-    s_scan[threadIdx.x] += add;
-    __syncthreads();
-  }
-  double running = s_before + (threadIdx.x ? s_scan[threadIdx.x - 1] : 0.0);
+  // ---- the chunk: a thread has one, or a run of them (a vocabulary of more than four million)
+  const int per = (a.chunks + kDrawThreads - 1) / kDrawThreads, from = min(t * per, a.chunks), to = min(from + per, a.chunks);
+  double mine = 0.0, total = 0.0, before = 0.0, found_before = 0.0, last_before = 0.0;
   int found = 0x7fffffff, last = -1;
+  if (t == 0) { s_chunk = 0x7fffffff; s_last = -1; s_token = 0x7fffffff; }
+  const double* left = a.left + size_t(seq) * a.chunks;
+  const ChunkStat* stats = a.stats + size_t(d.row) * a.chunks;
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
+    auto mass = [&](int c) {      // the second turn: nothing is left of p - q, and the next token comes from p
+      return turn == 0 ? left[c] : stats[c].top > -INFINITY ? stats[c].sum * weight(stats[c].top, double(d.p_top), d.degree) * d.p_scale : 0.0;
+    };
+    mine = 0.0;
+#pragma unroll 1
+    for (int c = from; c < to; ++c) mine += mass(c);
+    before = sum_before(mine, s_scratch, total);
+    double running = before;
+#pragma unroll 1
+    for (int c = from; c < to; ++c) {
+      const double m = per == 1 ? mine : mass(c);
+      if (m > 0.0) {
+        last = c;
+        last_before = running;
+        if (running + m > d.u * total && found == 0x7fffffff) { found = c; found_before = running; }
+      }
+      running += m;
+    }
+    if (total > 0.0 || d.kind == 0) break;
+    d.kind = 0;      // (a draft that neither side allows, under equal rows)
+  }
+  const double limit = d.u * total;
+  if (found != 0x7fffffff) atomicMin(&s_chunk, found);
+  __syncthreads();
+  int chunk = s_chunk;
+  if (chunk == 0x7fffffff) {      // a limit that rounding has put at the very end: the last chunk of any weight
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    chunk = s_last;
+  }
+  if (chunk < 0) {
+    if (t == 0) a.next[seq] = -1;
+    return;
+  }
+  if (chunk >= from && chunk < to) s_before = found == chunk ? found_before : last_before;
+  // ---- the token
+  const bool drawn = d.kind == 1 && d.draft_row >= 0;
+  const T* row = static_cast<const T*>(a.logits) + size_t(d.row) * a.vocab;
+  const T* draft_row = drawn ? static_cast<const T*>(a.draft_logits) + size_t(d.draft_row) * a.vocab : row;
+  const int begin = chunk * kVerifyChunk + 4 * t;
+  float p[4], q[4];
+  if (VEC) {
+    load_four(row, begin, a.vocab, p);
+    load_four(draft_row, begin, a.vocab, q);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 4; ++j) {
+      p[j] = begin + j < a.vocab ? to_float(row[begin + j]) : -INFINITY;
+      q[j] = begin + j < a.vocab ? to_float(draft_row[begin + j]) : -INFINITY;
+    }
+  }
+  double w[4], in_chunk;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = left_of(d, drawn, d.degree, p[j], q[j], begin + j);
+  double running = sum_before(((w[0] + w[1]) + w[2]) + w[3], s_scratch, in_chunk) + s_before;
+  found = 0x7fffffff;
+  last = -1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
     running += w[j];
     if (w[j] > 0.0) {
       last = begin + j;
-      if (running > s_limit && found == 0x7fffffff) found = begin + j;
+      if (running > limit && found == 0x7fffffff) found = begin + j;
     }
   }
   if (found != 0x7fffffff) atomicMin(&s_token, found);
-  if (last >= 0) atomicMax(&s_last, last);
   __syncthreads();
-  // (a limit that rounding has put at the chunk's very end: its last token of any weight)
-  if (threadIdx.x == 0) a.next[seq] = s_token != 0x7fffffff ? s_token : s_last;
+  if (s_token == 0x7fffffff) {      // likewise within the chunk
+    if (t == 0) s_last = -1;
+    __syncthreads();
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    if (t == 0) a.next[seq] = s_last;
+  } else if (t == 0) {
+    a.next[seq] = s_token;
+  }
 }
 
 int chunks_of(int vocab) { return (vocab + kVerifyChunk - 1) / kVerifyChunk; }
@@ -292,10 +434,13 @@ size_t verify_bytes(int rows, int sequences, int vocab) {
   return 2 * size_t(rows) * c * sizeof(ChunkStat) + size_t(sequences) * c * sizeof(double) + size_t(sequences) * sizeof(Decision);
 }
 
-template <typename T> int launch_verify(hipStream_t s, const VerifyArgs& a) {
-  verify_stats_kernel<T><<<dim3(a.chunks, a.rows * (a.draft_logits ? 2 : 1)), 256, 0, s>>>(a);
-  verify_decide_kernel<T><<<dim3(a.chunks, a.sequences), 256, 0, s>>>(a);
-  if (a.temperature) verify_draw_kernel<T><<<a.sequences, 256, 0, s>>>(a);
+template <typename T, bool VEC> int launch_verify(hipStream_t s, const VerifyArgs& a) {
+  verify_stats_kernel<T, VEC><<<dim3(a.chunks, a.rows * (a.draft_logits ? 2 : 1)), 256, 0, s>>>(a);
+  verify_decide_kernel<T><<<a.sequences, 512, 0, s>>>(a);
+  if (a.temperature) {
+    verify_left_kernel<T, VEC><<<dim3(a.chunks, a.sequences), 256, 0, s>>>(a);
+    verify_draw_kernel<T, VEC><<<a.sequences, kDrawThreads, 0, s>>>(a);
+  }
   return check_launch("sp_verify_drafts");
 }
 
@@ -331,5 +476,10 @@ extern "C" int sp_verify_drafts(void* stream, int dtype, const void* logits, int
   a.stats = static_cast<ChunkStat*>(workspace);
   a.left = reinterpret_cast<double*>(a.stats + 2 * size_t(rows) * a.chunks);
   a.decisions = reinterpret_cast<Decision*>(a.left + size_t(sequences) * a.chunks);
-  return dtype == kF32 ? launch_verify<float>((hipStream_t)stream, a) : launch_verify<bf16_t>((hipStream_t)stream, a);
+  // rows of whole groups of four that start where four lie in one load
+  const uintptr_t starts_at = reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(a.draft_logits);
+  const bool vec = vocab % 4 == 0 && starts_at % (dtype == kF32 ? 16 : 8) == 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == kF32) return vec ? launch_verify<float, true>(s, a) : launch_verify<float, false>(s, a);
+  return vec ? launch_verify<bf16_t, true>(s, a) : launch_verify<bf16_t, false>(s, a);
 }

@@ -61,12 +61,16 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _here(what: str, *tensors) -> None:
-    """Every tensor without gaps on the current device, whose stream the launch goes to."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+def _here(what: str, *tensors) -> int:
+    """Every tensor (the first is there) without gaps on the current device; the stream to launch on.  (The stream by its raw handle: a
+    stream object and the question whether there is a GPU at all cost 6 us a call, as much as the launch.)"""
+    device = tensors[0].get_device()
     for t in tensors:
         if t is not None and (t.get_device() != device or device < 0 or not t.is_contiguous()):
             raise KernelError(f"{what}: operands must be contiguous and live on the current GPU; got {tuple(t.shape)} on {t.device}.")
+    if device != torch.cuda.current_device():
+        raise KernelError(f"{what}: operands on GPU {device}, but the current one is {torch.cuda.current_device()}.")
+    return torch._C._cuda_getCurrentRawStream(device) if _scope_stream is None else _scope_stream
 
 
 # Variants of an operation that a part may ask for, as the C interface numbers them.  Only the listed ones have
@@ -612,21 +616,21 @@ def q4_quantize(w: torch.Tensor, group: int, scale_dtype: torch.dtype = torch.bf
     """(codes, scales) of w [N, K] (float32 or bfloat16): scales [N, ceil(K / group)] = max |w| of the group / 7, rounded to `scale_dtype`;
     codes uint8 [N, ceil(K / 2)], two a byte, the first in the low half: round(w / scale) + 8, in 0 .. 15.  A group that holds NaN or an
     infinity has that as its scale."""
-    _here("q4_quantize", w)
+    stream = _here("q4_quantize", w)
     if w.dim() != 2 or scale_dtype not in _CODES:
         raise KernelError(f"q4_quantize: a matrix and scales in float32 or bfloat16 expected, got {tuple(w.shape)} and {scale_dtype}")
     N, K = w.shape
     groups = _q4_sizes(N, K, group)
     codes = torch.empty(N, (K + 1) // 2, dtype=torch.uint8, device=w.device)
     scales = torch.empty(N, groups, dtype=scale_dtype, device=w.device)
-    check(library().sp_q4_quantize(_stream(), _code(w, "weights"), w.data_ptr(), N, K, group, codes.data_ptr(), _CODES[scale_dtype], scales.data_ptr()))
+    check(library().sp_q4_quantize(stream, _code(w, "weights"), w.data_ptr(), N, K, group, codes.data_ptr(), _CODES[scale_dtype], scales.data_ptr()))
     return codes, scales
 
 
 def q4_pack(codes: torch.Tensor, scales: torch.Tensor, group: int, cols: int | None = None) -> Q4Matrix:
     """Lays codes and scales (as `q4_quantize` makes them) out for `gemm_q4`; once, when a model is loaded.  `cols`: K, by default
     twice the bytes of a row (an odd K has to be said)."""
-    _here("q4_pack", codes, scales)
+    stream = _here("q4_pack", codes, scales)
     if codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dim() != 2:
         raise KernelError(f"q4_pack: codes uint8 [N, K / 2] and scales [N, groups] expected, got {tuple(codes.shape)} {codes.dtype} and {tuple(scales.shape)}")
     N, K = codes.shape[0], 2 * codes.shape[1] if cols is None else int(cols)
@@ -635,21 +639,21 @@ def q4_pack(codes: torch.Tensor, scales: torch.Tensor, group: int, cols: int | N
         raise KernelError(f"q4_pack: [{N}, {K}] in groups of {group} has {(K + 1) // 2} bytes and {groups} scales a row; got {tuple(codes.shape)} and {tuple(scales.shape)}")
     words = torch.empty(library().sp_q4_words(N, K), dtype=torch.int32, device=codes.device)
     packed = torch.empty(groups, (N + 15) // 16 * 16, dtype=scales.dtype, device=codes.device)
-    check(library().sp_q4_pack(_stream(), codes.data_ptr(), _code(scales, "scales"), scales.data_ptr(), N, K, group, words.data_ptr(), packed.data_ptr()))
+    check(library().sp_q4_pack(stream, codes.data_ptr(), _code(scales, "scales"), scales.data_ptr(), N, K, group, words.data_ptr(), packed.data_ptr()))
     return Q4Matrix(N, K, group, words, packed)
 
 
 def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False) -> None:
     """out = a @ w.T (+ bias) of a's dtype (float32 or bfloat16); with accumulate, out (float32) += a @ w.T (+ bias).  Made for few tokens: the
     weights are read once for every 64 (float32: 32)."""
-    _here("gemm_q4", a, w.words, w.scales, out, bias)
+    stream = _here("gemm_q4", a, w.words, w.scales, out, bias)
     if a.dim() != 2 or a.shape[1] != w.cols or tuple(out.shape) != (a.shape[0], w.rows):
         raise KernelError(f"gemm_q4: shapes do not fit: a {tuple(a.shape)}, w [{w.rows}, {w.cols}], out {tuple(out.shape)}")
     if out.dtype != (torch.float32 if accumulate else a.dtype):
         raise KernelError(f"gemm_q4: an output of {out.dtype}; a product of {a.dtype} is stored as that or added to float32")
     if bias is not None and bias.numel() != w.rows:
         raise KernelError(f"gemm_q4: bias has {bias.numel()} values for {w.rows} columns")
-    check(library().sp_gemm_q4(_stream(), _code(a, "input"), a.data_ptr(), w.words.data_ptr(), _CODES[w.scales.dtype], w.scales.data_ptr(),
+    check(library().sp_gemm_q4(stream, _code(a, "input"), a.data_ptr(), w.words.data_ptr(), _CODES[w.scales.dtype], w.scales.data_ptr(),
                                _code(bias, "bias") if bias is not None else 0, _ptr(bias), int(accumulate), _code(out, "output"),
                                out.data_ptr(), a.shape[0], w.rows, w.cols, w.group))
 
@@ -962,6 +966,11 @@ def attention(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_pool: torc
     return False
 
 
+@functools.lru_cache(maxsize=4096)
+def _shared_workspace_floats(*sizes: int) -> int:
+    return library().sp_attention_shared_workspace_floats(*sizes)
+
+
 MAX_SHARED_HEAD_DIM = 256      # the largest head size that attention_shared takes
 
 
@@ -987,7 +996,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     if nkv <= 0 or nq <= 0 or nq % nkv or not 0 < hd <= MAX_SHARED_HEAD_DIM:
         raise KernelError(f"attention_shared: {nq} query heads of {hd} in {nkv} groups: heads of 1..{MAX_SHARED_HEAD_DIM} that divide into the groups expected")
     tiles, n_tiles = batch.lists["tiles_all_16"]
-    _here("attention_shared", q, k_pool, v_pool, block_tables, out, sinks, prefix_table, batch.q_start, batch.q_len, batch.ctx_len,
+    stream = _here("attention_shared", q, k_pool, v_pool, block_tables, out, sinks, prefix_table, batch.q_start, batch.q_len, batch.ctx_len,
           tiles if n_tiles else None)
     if q.dim() != 2 or out.dim() != 2 or out.shape[1] != nq * hd or q.shape[0] < out.shape[0] or q.dtype != out.dtype \
             or not nq * hd <= q_stride <= q.shape[1]:
@@ -1017,13 +1026,11 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     T = out.shape[0]
     if n_tiles > T:
         raise KernelError(f"attention_shared: {n_tiles} tiles of queries for {T} rows")
-    lib = library()
-    need = lib.sp_attention_shared_workspace_floats(code, hd, nq, nkv, T, n_tiles, prefix, max_ctx)
+    need = _shared_workspace_floats(code, hd, nq, nkv, T, n_tiles, prefix, max_ctx)
     ws = workspace(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
-    _here("attention_shared", ws)
-    if ws.dtype != torch.float32 or ws.numel() < need or ws.data_ptr() % 16:
+    if ws.dtype != torch.float32 or ws.numel() < need or ws.data_ptr() % 16 or ws.device != q.device or not ws.is_contiguous():
         raise KernelError(f"attention_shared: the workspace must hold {need} float32 values at a multiple of 16 bytes")
-    check(lib.sp_attention_shared(_stream(), code, q.data_ptr(), q_stride, k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
+    check(library().sp_attention_shared(stream, code, q.data_ptr(), q_stride, k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
                                   block_tables.shape[1], prefix_table.data_ptr(), prefix, batch.q_start.data_ptr(), batch.q_len.data_ptr(),
                                   batch.ctx_len.data_ptr(), tiles.data_ptr(), n_tiles, max_ctx, T, ws.data_ptr(), need, out.data_ptr(), nq, nkv,
                                   hd, page_size, num_pages, float(scale), float(softcap), _ptr(sinks)))
@@ -1689,7 +1696,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, starts: torch.Tens
     holds while it is the lowest index of the maximum, and the next token is that index.  A logit of -infinity is a token that is not
     allowed; a deciding row with NaN or +infinity, or without any token allowed, gives next_token -1, as `sample` does.
     starts, lens: int32, one a sequence; uniform: float32 in [0, 1), one a row; temperature: float32, one a sequence; accepted, next_token: int32."""
-    _here("verify_drafts", logits, tokens, starts, lens, uniform, accepted, next_token, workspace, temperature, draft_logits, draft_rows)
+    stream = _here("verify_drafts", logits, tokens, starts, lens, uniform, accepted, next_token, workspace, temperature, draft_logits, draft_rows)
     code = _code(logits, "logits")
     if logits.dim() != 2:
         raise KernelError(f"verify_drafts: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
@@ -1710,7 +1717,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, starts: torch.Tens
         raise KernelError(f"verify_drafts: draft logits {tuple(draft_logits.shape)} {draft_logits.dtype} do not fit logits {tuple(logits.shape)} {logits.dtype}")
     if workspace.dtype != torch.float32:
         raise KernelError("verify_drafts: the workspace must be float32")
-    check(library().sp_verify_drafts(_stream(), code, logits.data_ptr(), R, V, tokens.data_ptr(), starts.data_ptr(), lens.data_ptr(), n,
+    check(library().sp_verify_drafts(stream, code, logits.data_ptr(), R, V, tokens.data_ptr(), starts.data_ptr(), lens.data_ptr(), n,
                                      _ptr(uniform), _ptr(temperature), _ptr(draft_logits), 0 if draft_logits is None else draft_logits.shape[0],
                                      _ptr(draft_rows), accepted.data_ptr(), next_token.data_ptr(), workspace.data_ptr(), workspace.numel()))
 
