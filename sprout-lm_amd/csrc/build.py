@@ -17,10 +17,10 @@ ARCH = "gfx950"
 # -packed-fp32-ops is switched off: the compiler must not form packed float32 instructions.
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
          "-packed-fp32-ops", "-Wno-unused-result"]
-# Attention rescales its MFMA accumulators with vector instructions at every step, and so does the delta rule's state;
+# Attention rescales its MFMA accumulators with vector instructions at every step, so does the delta rule's state, and 4-bit products scale every group's sums;
 # kept in AGPRs each such step would cost a move out and a move back, so these kernels take the VGPR form of MFMA.
 FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("attention_mfma.hip", "attention_mfma_sigmoid.hip", "attention_mixed.hip",
-                                                                              "attention_mfma_wide.hip", "attention_mfma_wide_sigmoid.hip", "attention_rows.hip", "attention_split.hip", "attention_shared.hip",
+                                                                              "attention_mfma_wide.hip", "attention_mfma_wide_sigmoid.hip", "attention_rows.hip", "attention_split.hip", "attention_shared.hip", "gemm_q4.hip", "gemm_q4_staged_bf16.hip", "gemm_q4_staged_f32.hip",
                                                                               "delta.hip")}
 
 

@@ -1,166 +1,108 @@
-// Products with weights of 4 bits and a scale per group of K, for the few tokens of decode and verify steps.
-//
-//   out[t, n] = sum over groups g of scale[n, g] * sum over k in g of (code[n, k] - 8) x[t, k]   (+ bias[n])       code 0 .. 15
-//
-// The weights' bytes bound it: they are laid out once (sp_q4_pack) so that a wave's 16-byte loads are the matrix instruction's operands,
-// a lane's four words being its eight codes of each of four steps of 32 along K, of 16 rows of weights.  A code becomes a bfloat16
-// number without a conversion: put into bits 3 to 6 of the mantissa of 16.0 it reads 16 + code, exactly, two codes an instruction
-// and its shift.  The 24 too much is taken off by the matrix cores: the sums of a group start from the product of x with rows of -24,
-// which is the same for all rows of weights and costs one product beside those of a wave's 16 NT rows.  So the codes, which are
-// whole numbers, meet x unrounded; the sums of a group are float32 and multiplied by the scale in float32.
-// float32 x is taken as the sum of three bfloat16 numbers, which holds all its bits: three products each.
-#include "mfma.h"
-#include "sprout_hip.h"
+// Products with 4-bit weights for a few tokens, their packing, and the entry points.
+#include "gemm_q4.h"
 
 namespace sprout {
 
-// bfloat16 x and results are handled as their bits
-template <> __device__ __forceinline__ uint16_t from_float<uint16_t>(float f) { return f32_to_bf16_bits(f); }
+using namespace q4;
 
 namespace {
 
-constexpr int kBlockK = 128;      // k of one 16-byte load of a lane: four steps of 32
-
-struct Q4Args {
-  const void* x;
-  const uint32_t* words;      // [rows / 16][K / 128][64 lanes][4]
-  const void* scales;         // [groups][rows up to a multiple of 16]
-  const void* bias;
-  void* out;
-  int T, N, K, blocks, groups, padded;      // blocks: of 128 along K; padded: N up to a multiple of 16
-  int scales_bf16, bias_bf16, accumulate;
-};
-
-__device__ __forceinline__ bf16x8 codes_plus_16(uint32_t w) {
-  constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
-  return as_bf16x8(make_uint4(((w << 3) & kMask) | kSixteen, ((w >> 1) & kMask) | kSixteen, ((w >> 5) & kMask) | kSixteen, ((w >> 9) & kMask) | kSixteen));
-}
-__device__ __forceinline__ float4 four_scales(const void* scales, int bf16, size_t at) {
-  if (bf16) {
-    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(scales) + at);
-    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
-  }
-  return *reinterpret_cast<const float4*>(static_cast<const float*>(scales) + at);
-}
-
-// Eight numbers of token t from k on, as PARTS operands.  VEC: rows start at whole 16 bytes and K is whole eights.
-template <bool VEC>
-__device__ __forceinline__ void x_operand(const uint16_t* x, int t, int k, int K, bf16x8 (&p)[1]) {
-  const uint16_t* src = x + size_t(t) * K + k;
-  if (VEC) {
-    p[0] = as_bf16x8(k < K ? ldg128(src) : make_uint4(0, 0, 0, 0));
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = (k + 2 * j < K ? uint32_t(src[2 * j]) : 0u) | (k + 2 * j + 1 < K ? uint32_t(src[2 * j + 1]) << 16 : 0u);
-    p[0] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-  }
-}
-template <bool VEC>
-__device__ __forceinline__ void x_operand(const float* x, int t, int k, int K, bf16x8 (&p)[3]) {
-  const float* src = x + size_t(t) * K + k;
-  float f[8];
-  if (VEC) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    if (k < K) { a = *reinterpret_cast<const float4*>(src); b = *reinterpret_cast<const float4*>(src + 4); }
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = k + j < K ? src[j] : 0.f;
-  }
-  uint4 q[3];
-  three_parts(f[0], f[1], q[0].x, q[1].x, q[2].x);
-  three_parts(f[2], f[3], q[0].y, q[1].y, q[2].y);
-  three_parts(f[4], f[5], q[0].z, q[1].z, q[2].z);
-  three_parts(f[6], f[7], q[0].w, q[1].w, q[2].w);
-#pragma unroll
-  for (int i = 0; i < 3; ++i) p[i] = as_bf16x8(q[i]);
-}
-
-// A block of four waves: NT tiles of 16 rows of weights by TT tiles of 16 tokens, the waves take turns along K and join in LDS.
-// X: x's type; STEPS: steps of 32 in a group.
-template <typename X, int NT, int TT, int STEPS, bool VEC>
+// X, S: x's type and the scales'; STEPS: steps of 32 in a group.
+template <typename X, typename S, int NT, int STEPS, bool VEC>
 __global__ __launch_bounds__(256) void gemm_q4_kernel(Q4Args a) {
-  constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
-  __shared__ floatx4 s_sums[3][NT * TT][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 15, lj = lane >> 4;
-  const int tile0 = blockIdx.x * NT, tiles = a.padded / 16, t0 = blockIdx.y * 16 * TT;
-  floatx4 total[NT][TT];
+  constexpr bool kF32 = sizeof(X) == 4;
+  constexpr int PARTS = kF32 ? 3 : 1, GROUPS = 4 / STEPS;
+  __shared__ floatx4 s_sums[3][NT][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lj = lane >> 4;
+  const int tile0 = blockIdx.x * NT, tiles = a.padded / 16, token = blockIdx.y * 16 + lr, split = blockIdx.z;
+  const int k_from = int((long long)(a.blocks) * split / a.splits), k_to = int((long long)(a.blocks) * (split + 1) / a.splits);
+  const floatx4 zero = floatx4{0.f, 0.f, 0.f, 0.f};
+  floatx4 total[NT], sum[NT], off = zero;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int t = 0; t < TT; ++t) total[n][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < NT; ++n) total[n] = sum[n] = zero;
   const bf16x8 minus24 = as_bf16x8(make_uint4(0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u));
-  for (int kb = wave; kb < a.blocks; kb += 4) {
-    uint4 w[NT];
+  const X* x_row = static_cast<const X*>(a.x) + size_t(min(token, a.T - 1)) * a.K;
+  const uint32_t* words[NT];
+  const S* scales[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) w[n] = ldg128(a.words + (size_t(min(tile0 + n, tiles - 1)) * a.blocks + kb) * 256 + 4 * lane);
+  for (int n = 0; n < NT; ++n) {
+    const int tile = min(tile0 + n, tiles - 1);
+    words[n] = a.words + size_t(tile) * a.blocks * 256 + 4 * lane;
+    scales[n] = static_cast<const S*>(a.scales) + 16 * tile + 4 * lj;
+  }
+  // Loads come back in the order in which they were asked for: whoever waits for x waits for weights asked for before it.  So everything
+  // of a block of 128 along K is asked for a whole block before, each part where its predecessor has been used.
+  uint4 w[NT], w_next[NT];
+  typename RawOf<X>::type raw[4];
+  ScaleBits<S> scale[GROUPS][NT];
+  auto load_words = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int gs = 0; gs < 4 / STEPS; ++gs) {
-      bf16x8 b[TT][STEPS][PARTS];
+    for (int n = 0; n < NT; ++n) w_next[n] = ldg128(words[n] + size_t(kb) * 256);
+  };
+  auto load_x = [&](int kb, int s) __attribute__((always_inline)) { x_load<VEC>(x_row, 128 * kb + 32 * s + 8 * lj, a.K, raw[s]); };
+  auto load_scales = [&](int kb, int g) __attribute__((always_inline)) {      // (behind the last group x is zero)
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
+    for (int n = 0; n < NT; ++n) load_scale(scales[n] + size_t(min(GROUPS * kb + g, a.groups - 1)) * a.padded, scale[g][n]);
+  };
+  int kb = k_from + wave;
+  if (kb < k_to) {
+    load_words(kb);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-          x_operand<VEC>(static_cast<const X*>(a.x), min(t0 + 16 * t + lr, a.T - 1), kBlockK * kb + 32 * (gs * STEPS + s) + 8 * lj, a.K, b[t][s]);
-      floatx4 off[TT];
+    for (int s = 0; s < 4; ++s) {
+      load_x(kb, s);
+      if (s % STEPS == 0) load_scales(kb, s / STEPS);
+    }
+  }
+  for (; kb < k_to; kb += 4) {
+    const int kb_next = min(kb + 4, k_to - 1);      // (behind the wave's last: something that is there)
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        off[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NT; ++n) w[n] = w_next[n];
+    load_words(kb_next);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int p = PARTS - 1; p >= 0; --p) off[t] = mfma16(minus24, b[t][s][p], off[t]);
-      }
-      const int group = min((4 * kb) / STEPS + gs, a.groups - 1);      // (behind the last group x is zero)
+    for (int s = 0; s < 4; ++s) {
+      bf16x8 b[PARTS];
+      x_operands(raw[s], b);
+      if (!kF32) off = mfma16(minus24, b[0], s % STEPS == 0 ? zero : off);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float4 scale = four_scales(a.scales, a.scales_bf16, size_t(group) * a.padded + 16 * min(tile0 + n, tiles - 1) + 4 * lj);
-        const uint32_t words[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
-        bf16x8 c[STEPS];
+        const bf16x8 c = weights_operand(s == 0 ? w[n].x : s == 1 ? w[n].y : s == 2 ? w[n].z : w[n].w, X());
+        floatx4 v = s % STEPS != 0 ? sum[n] : !kF32 && STEPS == 1 ? off : zero;
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) c[s] = codes_plus_16(words[gs * STEPS + s]);
+        for (int p = PARTS - 1; p >= 0; --p) v = mfma16(c, b[p], v);
+        sum[n] = v;
+      }
+      load_x(kb_next, s);
+      if (s % STEPS == STEPS - 1) {
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          floatx4 sum = off[t];
-#pragma unroll
-          for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int p = PARTS - 1; p >= 0; --p) sum = mfma16(c[s], b[t][s][p], sum);
-          total[n][t][0] += scale.x * sum[0];
-          total[n][t][1] += scale.y * sum[1];
-          total[n][t][2] += scale.z * sum[2];
-          total[n][t][3] += scale.w * sum[3];
+        for (int n = 0; n < NT; ++n) {
+          const float4 f = scale_values(scale[s / STEPS][n]);
+          const floatx4 v = !kF32 && STEPS > 1 ? sum[n] + off : sum[n];
+          total[n][0] += f.x * v[0];
+          total[n][1] += f.y * v[1];
+          total[n][2] += f.z * v[2];
+          total[n][3] += f.w * v[3];
         }
+        load_scales(kb_next, s / STEPS);
       }
     }
   }
   if (wave > 0) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int t = 0; t < TT; ++t) s_sums[wave - 1][n * TT + t][lane] = total[n][t];
+    for (int n = 0; n < NT; ++n) s_sums[wave - 1][n][lane] = total[n];
   }
   __syncthreads();
-  if (wave > 0) return;
+  if (wave > 0 || token >= a.T) return;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const floatx4 v = total[n][t] + s_sums[0][n * TT + t][lane] + s_sums[1][n * TT + t][lane] + s_sums[2][n * TT + t][lane];
-      const int token = t0 + 16 * t + lr;
-      if (token >= a.T) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * (tile0 + n) + 4 * lj + r;
-        if (row >= a.N) continue;
-        float y = v[r];
-        if (a.bias) y += a.bias_bf16 ? to_float(static_cast<const bf16_t*>(a.bias)[row]) : static_cast<const float*>(a.bias)[row];
-        const size_t at = size_t(token) * a.N + row;
-        if (a.accumulate) static_cast<float*>(a.out)[at] += y;
-        else static_cast<X*>(a.out)[at] = from_float<X>(y);
-      }
-    }
+    store_four<X>(a, split, token, 16 * (tile0 + n) + 4 * lj, ((total[n] + s_sums[0][n][lane]) + s_sums[1][n][lane]) + s_sums[2][n][lane]);
+}
+
+template <typename X> __global__ __launch_bounds__(256) void gemm_q4_join_kernel(Q4Args a) {
+  const size_t i = size_t(blockIdx.x) * 256 + threadIdx.x, results = size_t(a.T) * a.N;
+  if (i >= results) return;
+  float y = 0.f;
+  for (int s = 0; s < a.splits; ++s) y += a.parts[s * results + i];
+  store_result<X>(a, int(i / a.N), int(i % a.N), y);
 }
 
 // Codes two a byte along K (the first in the low half) -> the words of sp_gemm_q4; scales [N, groups] -> [groups, N padded].
@@ -212,16 +154,59 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const W* __restrict__ 
   if (lane == 0) scales[i] = stored;
 }
 
-template <typename X, int NT, int TT, bool VEC> void launch_q4(hipStream_t s, const Q4Args& a, int steps) {
-  const dim3 grid((a.padded / 16 + NT - 1) / NT, (a.T + 16 * TT - 1) / (16 * TT));
-  if (steps == 1) gemm_q4_kernel<X, NT, TT, 1, VEC><<<grid, 256, 0, s>>>(a);
-  else if (steps == 2) gemm_q4_kernel<X, NT, TT, 2, VEC><<<grid, 256, 0, s>>>(a);
-  else gemm_q4_kernel<X, NT, TT, 4, VEC><<<grid, 256, 0, s>>>(a);
+// Which kernel, how many tiles of 16 rows and tokens a wave or block takes, and over how many blocks K is split (bfloat16 unless float32 is
+// named; us, groups of 128 where nothing else stands; sizes as rows x K).
+//  - x through LDS costs barriers and pays where x is read often and the weights are many: 55,296 x 5,120, 64 tokens of group 32, 85.8
+//    against more than 150; 3,584 x 18,944, 40 tokens of group 64, 29.9 against 33.0; float32 37,888 x 3,584 of group 64, one token, 29.4
+//    against 36.9.  Up to 16 tokens (16 of 37,888 x 3,584: 21.8 without it, 22.8 with) and where 16 Mi weights or fewer are spread over few
+//    blocks (33 tokens of 9,728 x 896: 7.9 against 10.8) it is left out.
+//  - Without it, more tiles a wave read x less often, fewer keep more blocks in flight: one token of 37,888 rows 17.6 with two tiles, 18.8
+//    with four, 21.9 with one; 16 tokens 21.8 with four, 27.3 with two; 3,584 x 3,584 7.1 with one, 7.8 with two.  A long K is better split
+//    over blocks of four tiles (16 tokens of 3,584 x 18,944: 18.8, two tiles 22.6), a short one over blocks of one tile (one token
+//    of 896 x 4,864: 6.5 in four parts, 7.1 in one; in eight 7.3).
+//  - With it, a wave's two tiles of rows become four where the rows are many (64 tokens of 55,296: 67.3 against 74.2) and 48 or 64 tokens
+//    share a pass; float32's three parts leave room for 32 tokens (64 tokens of 37,888 x 3,584: 82.7, by 16 each 90.8; 40 tokens
+//    leave half of the second 32 empty: 71.1 by 16, 79.6 by 32).  K is split until each compute unit has two blocks (five of float32).
+Q4Plan q4_plan(int x_dtype, int T, int N, int K) {
+  Q4Plan p;
+  const bool f32 = x_dtype == kF32, small = int64_t(N) * K <= 16 << 20;
+  const int tiles = (N + 15) / 16, blocks = (K + kBlockK - 1) / kBlockK, tokens = (T + 15) / 16;
+  p.staged = small ? T > 48 : f32 ? T > 4 || tiles >= 1024 : T > 16;
+  p.splits = 1;
+  if (p.staged) {
+    const int rounds = (tokens + 3) / 4;
+    p.token_tiles = f32 ? (tokens % 2 == 0 ? 2 : 1) : (tokens + rounds - 1) / rounds;
+    p.row_tiles = !f32 && p.token_tiles >= 3 && tiles >= 1024 ? 4 : 2;
+    const int64_t grid = int64_t(tiles + 4 * p.row_tiles - 1) / (4 * p.row_tiles) * ((tokens + p.token_tiles - 1) / p.token_tiles);
+    while (grid * p.splits * 4 < (f32 ? 1280 : 448) * 3 && p.splits < 16 && blocks >= 2 * p.splits) p.splits *= 2;
+  } else {
+    const int64_t units = int64_t(tiles) * tokens;
+    const bool long_k = units < 400 && blocks >= 64;
+    p.token_tiles = 1;
+    p.row_tiles = long_k ? 4 : T <= 4 ? (units >= 1024 ? 2 : 1) : units >= 600 ? 4 : units >= 400 ? 2 : 1;
+    const int64_t grid = int64_t(tiles + p.row_tiles - 1) / p.row_tiles * tokens;
+    while (grid * p.splits * 2 <= (long_k ? 512 : 256) && blocks >= 2 * p.splits * (long_k ? 16 : 8)) p.splits *= 2;
+  }
+  return p;
 }
-template <typename X> void launch_q4_of(hipStream_t s, const Q4Args& a, int steps, bool vec) {
-  if (vec) launch_q4<X, 1, 1, true>(s, a, steps);
-  else launch_q4<X, 1, 1, false>(s, a, steps);
+
+template <typename X, typename S, int NT, bool VEC> void launch_q4_steps(hipStream_t s, const Q4Args& a, int steps) {
+  const dim3 grid((a.padded / 16 + NT - 1) / NT, (a.T + 15) / 16, a.splits);
+  if (steps == 1) gemm_q4_kernel<X, S, NT, 1, VEC><<<grid, 256, 0, s>>>(a);
+  else if (steps == 2) gemm_q4_kernel<X, S, NT, 2, VEC><<<grid, 256, 0, s>>>(a);
+  else gemm_q4_kernel<X, S, NT, 4, VEC><<<grid, 256, 0, s>>>(a);
 }
+template <typename X, typename S> void launch_q4_of(hipStream_t s, const Q4Args& a, const Q4Plan& p, int steps, bool vec) {
+  if (!vec) launch_q4_steps<X, S, 1, false>(s, a, steps);
+  else if (p.staged && sizeof(X) == 4) gemm_q4_staged_f32(s, a, p, steps, sizeof(S) == 2);
+  else if (p.staged) gemm_q4_staged_bf16(s, a, p, steps, sizeof(S) == 2);
+  else if (p.row_tiles == 1) launch_q4_steps<X, S, 1, true>(s, a, steps);
+  else if (p.row_tiles == 2) launch_q4_steps<X, S, 2, true>(s, a, steps);
+  else launch_q4_steps<X, S, 4, true>(s, a, steps);
+  if (a.splits > 1) gemm_q4_join_kernel<X><<<unsigned((size_t(a.T) * a.N + 255) / 256), 256, 0, s>>>(a);
+}
+
+constexpr size_t kMostBlocks = (size_t(1) << 24) - 1;      // a launch has less than 2^32 threads
 
 bool q4_sizes(int N, int K, int group) { return N > 0 && K > 0 && (group == 32 || group == 64 || group == 128); }
 
@@ -239,7 +224,7 @@ extern "C" int sp_q4_pack(void* stream, const void* codes, int scale_dtype, cons
   SP_REQUIRE(codes && scales && words && packed_scales, "sp_q4_pack: null argument");
   const size_t total = size_t(sp_q4_words(N, K));
   const int groups = (K + group - 1) / group, padded = (N + 15) / 16 * 16, blocks = (K + kBlockK - 1) / kBlockK;
-  SP_REQUIRE(total / 256 < (size_t(1) << 31) && size_t(groups) * padded / 256 < (size_t(1) << 31) - 1, "sp_q4_pack: the matrix is too large");
+  SP_REQUIRE(total / 256 < kMostBlocks && size_t(groups) * padded / 256 < kMostBlocks, "sp_q4_pack: the matrix is too large");
   hipStream_t s = (hipStream_t)stream;
   q4_pack_kernel<<<(total + 255) / 256, 256, 0, s>>>(static_cast<const uint8_t*>(codes), static_cast<uint32_t*>(words), N, K, blocks, total);
   const unsigned grid = unsigned((size_t(groups) * padded + 255) / 256);
@@ -254,7 +239,7 @@ extern "C" int sp_q4_quantize(void* stream, int w_dtype, const void* w, int N, i
   SP_REQUIRE(w && codes && scales, "sp_q4_quantize: null argument");
   const int groups = (K + group - 1) / group;
   const size_t units = size_t(N) * groups;
-  SP_REQUIRE(units / 4 < (size_t(1) << 31) - 1, "sp_q4_quantize: the matrix is too large");
+  SP_REQUIRE(units / 4 < kMostBlocks, "sp_q4_quantize: the matrix is too large");
   const unsigned grid = unsigned((units + 3) / 4);
   hipStream_t s = (hipStream_t)stream;
   uint8_t* c = static_cast<uint8_t*>(codes);
@@ -265,8 +250,15 @@ extern "C" int sp_q4_quantize(void* stream, int w_dtype, const void* w, int N, i
   return check_launch("sp_q4_quantize");
 }
 
+extern "C" int64_t sp_gemm_q4_workspace_floats(int x_dtype, int T, int N, int K) {
+  if (T <= 0 || N <= 0 || K <= 0) return 0;
+  const int splits = q4_plan(x_dtype, T, N, K).splits;
+  return splits > 1 ? int64_t(splits) * T * N : 0;
+}
+
 extern "C" int sp_gemm_q4(void* stream, int x_dtype, const void* x, const void* words, int scale_dtype, const void* scales, int bias_dtype,
-                          const void* bias, int mode, int out_dtype, void* out, int T, int N, int K, int group) {
+                          const void* bias, int mode, int out_dtype, void* out, int T, int N, int K, int group, float* workspace,
+                          int64_t workspace_floats) {
   SP_REQUIRE(q4_sizes(N, K, group) && T >= 0, "sp_gemm_q4: T=%d N=%d K=%d group=%d (groups of 32, 64 or 128)", T, N, K, group);
   SP_REQUIRE((x_dtype == kF32 || x_dtype == kBF16) && (scale_dtype == kF32 || scale_dtype == kBF16) && (bias_dtype == kF32 || bias_dtype == kBF16),
              "sp_gemm_q4: unsupported dtypes %d, %d, %d", x_dtype, scale_dtype, bias_dtype);
@@ -274,14 +266,24 @@ extern "C" int sp_gemm_q4(void* stream, int x_dtype, const void* x, const void* 
   if (T == 0) return 0;
   SP_REQUIRE(x && words && scales && out, "sp_gemm_q4: null argument");
   SP_REQUIRE(reinterpret_cast<uintptr_t>(words) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 16 == 0, "sp_gemm_q4: packed weights must start at a multiple of 16 bytes");
-  SP_REQUIRE(T <= 65535 * 16, "sp_gemm_q4: %d tokens", T);
+  SP_REQUIRE(T <= 65535 * 16 && K < 1 << 25, "sp_gemm_q4: %d tokens, K=%d", T, K);      // (64 rows of x within 32 bits)
   Q4Args a;
   a.x = x; a.words = static_cast<const uint32_t*>(words); a.scales = scales; a.bias = bias; a.out = out;
   a.T = T; a.N = N; a.K = K; a.blocks = (K + kBlockK - 1) / kBlockK; a.groups = (K + group - 1) / group; a.padded = (N + 15) / 16 * 16;
-  a.scales_bf16 = scale_dtype == kBF16; a.bias_bf16 = bias_dtype == kBF16; a.accumulate = mode == 1;
-  const int per = x_dtype == kF32 ? 4 : 8;
-  const bool vec = K % 8 == 0 && K % per == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  if (x_dtype == kF32) launch_q4_of<float>((hipStream_t)stream, a, group / 32, vec);
-  else launch_q4_of<uint16_t>((hipStream_t)stream, a, group / 32, vec);
+  a.bias_bf16 = bias_dtype == kBF16; a.accumulate = mode == 1;
+  const Q4Plan p = q4_plan(x_dtype, T, N, K);
+  const int64_t need = sp_gemm_q4_workspace_floats(x_dtype, T, N, K);
+  SP_REQUIRE(need == 0 || (workspace && workspace_floats >= need), "sp_gemm_q4: workspace of %lld floats is smaller than the %lld needed",
+             (long long)workspace_floats, (long long)need);
+  a.splits = p.splits;
+  a.parts = workspace;
+  a.fours = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 == 0;
+  const bool vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  hipStream_t s = (hipStream_t)stream;
+  const int steps = group / 32;
+  if (x_dtype == kF32 && scale_dtype == kF32) launch_q4_of<float, float>(s, a, p, steps, vec);
+  else if (x_dtype == kF32) launch_q4_of<float, uint16_t>(s, a, p, steps, vec);
+  else if (scale_dtype == kF32) launch_q4_of<uint16_t, float>(s, a, p, steps, vec);
+  else launch_q4_of<uint16_t, uint16_t>(s, a, p, steps, vec);
   return check_launch("sp_gemm_q4");
 }

@@ -491,10 +491,11 @@ int sp_verify_drafts(void* stream, int dtype, const void* logits, int rows, int 
 // sp_q4_quantize: codes [N, (K + 1) / 2], two a byte along K with the first in the low half, and scales [N, groups] of w [N, K]: scale =
 // max |w| / 7 rounded to scale_dtype, code = w / scale rounded to the nearest whole number.  sp_q4_pack: the same laid out for the product,
 // `words` sp_q4_words(N, K) of 32 bits, packed_scales [groups, N up to a multiple of 16].  sp_gemm_q4: out = x . w^T (+ bias) of x's dtype
-// (mode 0), or out (float32) += (mode 1); sums and scales are multiplied in float32.
+// (mode 0), or out (float32) += (mode 1); sums and scales are multiplied in float32.  workspace: sp_gemm_q4_workspace_floats numbers (0: none).
+int64_t sp_gemm_q4_workspace_floats(int x_dtype, int T, int N, int K);
 int64_t sp_q4_words(int N, int K);
 int sp_q4_quantize(void* stream, int w_dtype, const void* w, int N, int K, int group, void* codes, int scale_dtype, void* scales);
 int sp_q4_pack(void* stream, const void* codes, int scale_dtype, const void* scales, int N, int K, int group, void* words, void* packed_scales);
 int sp_gemm_q4(void* stream, int x_dtype, const void* x, const void* words, int scale_dtype, const void* scales, int bias_dtype,
-               const void* bias, int mode, int out_dtype, void* out, int T, int N, int K, int group);
+               const void* bias, int mode, int out_dtype, void* out, int T, int N, int K, int group, float* workspace, int64_t workspace_floats);
 }

@@ -643,9 +643,16 @@ def q4_pack(codes: torch.Tensor, scales: torch.Tensor, group: int, cols: int | N
     return Q4Matrix(N, K, group, words, packed)
 
 
-def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False) -> None:
+@functools.lru_cache(maxsize=4096)
+def gemm_q4_workspace_floats(dtype: torch.dtype, T: int, N: int, K: int) -> int:
+    """float32 values of workspace that `gemm_q4` wants for T tokens of `dtype` by a matrix [N, K]; 0: none."""
+    return library().sp_gemm_q4_workspace_floats(_CODES[dtype], T, N, K) if dtype in _CODES else 0
+
+
+def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False, workspace=None) -> None:
     """out = a @ w.T (+ bias) of a's dtype (float32 or bfloat16); with accumulate, out (float32) += a @ w.T (+ bias).  Made for few tokens: the
-    weights are read once for every 64 (float32: 32)."""
+    weights are read once for every 64.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new
+    one, where the product needs any); calls that may run at the same time need one each."""
     stream = _here("gemm_q4", a, w.words, w.scales, out, bias)
     if a.dim() != 2 or a.shape[1] != w.cols or tuple(out.shape) != (a.shape[0], w.rows):
         raise KernelError(f"gemm_q4: shapes do not fit: a {tuple(a.shape)}, w [{w.rows}, {w.cols}], out {tuple(out.shape)}")
@@ -653,9 +660,14 @@ def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor 
         raise KernelError(f"gemm_q4: an output of {out.dtype}; a product of {a.dtype} is stored as that or added to float32")
     if bias is not None and bias.numel() != w.rows:
         raise KernelError(f"gemm_q4: bias has {bias.numel()} values for {w.rows} columns")
+    need, ws = gemm_q4_workspace_floats(a.dtype, a.shape[0], w.rows, w.cols), None
+    if need:
+        ws = workspace(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=a.device)
+        if ws.dtype != torch.float32 or ws.numel() < need or ws.device != a.device or not ws.is_contiguous():
+            raise KernelError(f"gemm_q4: the workspace must hold {need} float32 values")
     check(library().sp_gemm_q4(stream, _code(a, "input"), a.data_ptr(), w.words.data_ptr(), _CODES[w.scales.dtype], w.scales.data_ptr(),
                                _code(bias, "bias") if bias is not None else 0, _ptr(bias), int(accumulate), _code(out, "output"),
-                               out.data_ptr(), a.shape[0], w.rows, w.cols, w.group))
+                               out.data_ptr(), a.shape[0], w.rows, w.cols, w.group, _ptr(ws), need))
 
 
 @functools.lru_cache(maxsize=4096)

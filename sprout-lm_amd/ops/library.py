@@ -128,7 +128,8 @@ def _declare(lib):
                              c_void, c_void, c_void, c_i64],
         "sp_q4_quantize": [c_void, c_int, c_void, c_int, c_int, c_int, c_void, c_int, c_void],
         "sp_q4_pack": [c_void, c_void, c_int, c_void, c_int, c_int, c_int, c_void, c_void],
-        "sp_gemm_q4": [c_void, c_int, c_void, c_void, c_int, c_void, c_int, c_void, c_int, c_int, c_void, c_int, c_int, c_int, c_int],
+        "sp_gemm_q4": [c_void, c_int, c_void, c_void, c_int, c_void, c_int, c_void, c_int, c_int, c_void, c_int, c_int, c_int, c_int, c_void,
+                       c_i64],
         "sp_probe_read": [c_void, c_void, c_i64, c_int, c_void],
         "sp_probe_mfma": [c_void, c_int, c_int, c_void, ctypes.POINTER(ctypes.c_double)],
     }
@@ -146,6 +147,8 @@ def _declare(lib):
     lib.sp_attention_shared_workspace_floats.restype = c_i64
     lib.sp_verify_workspace_floats.argtypes = [c_int] * 3
     lib.sp_verify_workspace_floats.restype = c_i64
+    lib.sp_gemm_q4_workspace_floats.argtypes = [c_int] * 4
+    lib.sp_gemm_q4_workspace_floats.restype = c_i64
     lib.sp_q4_words.argtypes = [c_int] * 2
     lib.sp_q4_words.restype = c_i64
     lib.sp_rglru_carry_floats.argtypes = [c_int] * 4

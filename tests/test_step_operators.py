@@ -37,8 +37,8 @@ def test_drafts_refuse_at_the_c_interface():
 
 def test_4_bit_products_refuse_at_the_c_interface():
     lib = ops.library()
-    #       stream dtype x  words dtype scales dtype bias mode dtype out T  N  K  group
-    good = [None, 1, 16, 16, 1, 16, 0, None, 0, 1, 16, 2, 20, 64, 32]
+    #       stream dtype x  words dtype scales dtype bias mode dtype out T  N  K  group workspace floats
+    good = [None, 1, 16, 16, 1, 16, 0, None, 0, 1, 16, 2, 20, 64, 32, None, 0]
     for at, value, match in ((1, 2, "dtypes"), (4, 2, "dtypes"), (6, 2, "dtypes"), (8, 1, "stores"), (8, 2, "stores"), (9, 0, "stores"), (11, -1, "groups"), (12, 0, "groups"), (13, 0, "groups"),
                              (14, 16, "groups"), (2, None, "null"), (5, None, "null"), (3, 20, "16 bytes"), (5, 8, "16 bytes"), (11, 1 << 21, "tokens")):
         refused(lib.sp_gemm_q4, *good[:at], value, *good[at + 1:], match=match)
