@@ -15,6 +15,11 @@
 // serve at a quarter of their rate: with 64 tokens that took four times as long as everything else.  With more tokens (gemm_q4_staged.h) x comes
 // through LDS, once for the four waves of a block.  Where rows of weights alone do not fill the chip several blocks (`splits`)
 // share out K and a second launch joins them, in a fixed order.
+//
+// One token of bfloat16 by 37,888 x 3,584 in groups of 64: 15.3 us, 4.6 TB/s of weights and scales, near what a copy reaches.  64 tokens by
+// 55,296 x 5,120 in groups of 32: 93 us, 390 TFLOP/s, bound by the vector unit: a group of 32 along K of one row and 16 tokens costs one
+// matrix instruction of 16 cycles, four float32 multiply-adds by the scale, 16 cycles, and of unpacking codes and scales 11 more
+// (in groups of 128: 67 us).  40 tokens of float32 by 3,584 x 18,944: 45 us, three products of bfloat16 each, 118 TFLOP/s of float32.
 #pragma once
 #include "mfma.h"
 #include "sprout_hip.h"
@@ -40,8 +45,10 @@ struct Q4Args {
 };
 
 __device__ __forceinline__ uint4 codes_plus_16(uint32_t w) {
-  constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
-  return make_uint4(((w << 3) & kMask) | kSixteen, ((w >> 1) & kMask) | kSixteen, ((w >> 5) & kMask) | kSixteen, ((w >> 9) & kMask) | kSixteen);
+  constexpr uint32_t kMask = 0x00780078u;
+  uint32_t sixteen = 0x41804180u;      // in a vector register: one of the two constants may be a scalar, then "and" and "or" are one instruction
+  asm("" : "+v"(sixteen));
+  return make_uint4(((w << 3) & kMask) | sixteen, ((w >> 1) & kMask) | sixteen, ((w >> 5) & kMask) | sixteen, ((w >> 9) & kMask) | sixteen);
 }
 __device__ __forceinline__ uint32_t less_24(uint32_t pair) {      // (whole numbers up to 8: nothing is lost in the upper halves)
   const float lo = __uint_as_float(pair << 16) - 24.f, hi = __uint_as_float(pair & 0xffff0000u) - 24.f;
