@@ -82,6 +82,7 @@ __device__ __forceinline__ double table_power(const double* table, double diff, 
 // the largest logits rounds by more than any difference.)
 __device__ __forceinline__ double degree_of(float temperature) { return 1.4426950408889634 / double(temperature); }
 __device__ __forceinline__ double weight(float l, double top, double degree) { return two_to((double(l) - top) * degree); }
+__device__ __forceinline__ bool rows_there(const VerifyArgs& a, int start, int len) { return len > 0 && start >= 0 && start <= a.rows - len; }
 __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int s) { return a.temperature ? a.temperature[s] : 0.f; }
 
 // Sixteen logits of a chunk to a thread: groups of four, 1,024 apart (VEC), or single ones 256 apart.  What lies behind the row is -infinity.
@@ -126,8 +127,8 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) { s_seq = -1; s_best = 0x7fffffff; }
   __syncthreads();
   for (int s = threadIdx.x; s < a.sequences; s += 256) {
-    const int at = place - a.starts[s];
-    if (at >= (drafter ? 1 : 0) && at < a.lens[s]) s_seq = s;
+    const int start = a.starts[s], len = a.lens[s];
+    if (rows_there(a, start, len) && place >= start + (drafter ? 1 : 0) && place - start < len) s_seq = s;
   }
   __syncthreads();
   const int seq = s_seq;
@@ -202,7 +203,12 @@ __global__ __launch_bounds__(512) void verify_decide_kernel(VerifyArgs a) {
   __shared__ int s_holds[kRows], s_next[kRows];
   const int seq = blockIdx.x, wave = threadIdx.x >> 6;
   const int start = a.starts[seq], len = a.lens[seq];
-  if (len <= 0 || start < 0 || start > a.rows - len) {      // rows that are not there
+  bool refused = !rows_there(a, start, len);
+  for (int s = threadIdx.x; s < a.sequences; s += 512) {
+    const int other = a.starts[s], n = a.lens[s];
+    if (s != seq && !refused && rows_there(a, other, n) && other < start + len && start < other + n) refused = true;
+  }
+  if (__syncthreads_or(refused)) {      // rows that are not there, or also another sequence's, whose temperature may differ
     if (threadIdx.x == 0) { a.accepted[seq] = 0; a.next[seq] = -1; a.decisions[seq].kind = 2; }
     return;
   }
@@ -466,13 +472,13 @@ extern "C" int sp_verify_drafts(void* stream, int dtype, const void* logits, int
   SP_REQUIRE(rows > 0 && rows <= 32767, "sp_verify_drafts: %d rows are outside 1..32767", rows);
   SP_REQUIRE(sequences <= 65535, "sp_verify_drafts: %d sequences are more than 65535", sequences);
   SP_REQUIRE(logits && tokens && starts && lens && accepted && next && (uniform || !temperature), "sp_verify_drafts: null argument");
-  SP_REQUIRE(!draft_logits == !draft_rows, "sp_verify_drafts: draft logits and the rows of the drafts go together");
+  SP_REQUIRE(!draft_logits == !draft_rows || (draft_rows && drafted == 0), "sp_verify_drafts: draft logits and the rows of the drafts go together");
   const int64_t need = sp_verify_workspace_floats(rows, sequences, vocab);
   SP_REQUIRE(workspace && workspace_floats >= need && reinterpret_cast<uintptr_t>(workspace) % 8 == 0,
              "sp_verify_drafts: workspace of %lld floats, %lld needed at a multiple of 8 bytes", (long long)workspace_floats, (long long)need);
   VerifyArgs a;
   a.logits = logits; a.draft_logits = temperature && drafted ? draft_logits : nullptr;
-  a.tokens = tokens; a.starts = starts; a.lens = lens; a.draft_rows = draft_logits ? draft_rows : nullptr;
+  a.tokens = tokens; a.starts = starts; a.lens = lens; a.draft_rows = draft_rows;
   a.uniform = uniform; a.temperature = temperature; a.accepted = accepted; a.next = next;
   a.rows = rows; a.drafted = drafted; a.sequences = sequences; a.vocab = vocab; a.chunks = chunks_of(vocab);
   a.stats = static_cast<ChunkStat*>(workspace);

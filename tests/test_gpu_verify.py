@@ -229,6 +229,27 @@ def test_from_a_graph_and_on_another_stream():
         assert (accepted.tolist(), following.tolist()) == definition(**data, temperature=torch.ones(4))
 
 
+@pytest.mark.parametrize("warmth", [None, 1.0], ids=["greedy", "drawn"])
+def test_rows_of_two_sequences(warmth):
+    """A row has one temperature: sequences that share rows are not answered, their neighbours are, also beside ranges that are not there."""
+    data = inputs(300, [2, 3, 1, 2], seed=6)
+    temperature = None if warmth is None else torch.full((4,), warmth)
+    accepted, following = call(**data, temperature=temperature)
+    wanted = definition(**data, temperature=temperature)
+    assert (accepted, following) == wanted
+    more = None if warmth is None else torch.full((8,), warmth)
+    rows = {**data, "starts": data["starts"] + [3, -1, 7, 4], "lens": data["lens"] + [2, 9, 2, 0]}      # rows 3 and 4 of the second; -1 ..; 7 and 8; none
+    accepted, following = call(**rows, temperature=more)
+    assert accepted == [wanted[0][0], 0, wanted[0][2], wanted[0][3], 0, 0, 0, 0]
+    assert following == [wanted[1][0], -1, wanted[1][2], wanted[1][3], -1, -1, -1, -1]
+
+
+def test_a_drafter_without_rows():
+    data = inputs(90, [3, 2], seed=8, drawn=0.0)
+    data["draft_logits"] = torch.zeros(0, 90)
+    assert call(**data, temperature=torch.ones(2)) == definition(**data, temperature=torch.ones(2))
+
+
 @pytest.mark.parametrize("what", ["dtype", "ints", "uniform", "missing", "pair", "draft", "workspace", "cpu", "rows"])
 def test_refusals(what):
     from sprout_lm_amd import ops
