@@ -481,7 +481,7 @@ int sp_attention_shared(void* stream, int dtype, const void* q, int q_stride, co
 // next token.  temperature (null: all 0) one a sequence, 0: greedy.  draft_logits [drafted, vocab] with draft_rows [rows]: the row that the
 // token at that place was drawn from, negative: not drawn (both null: none was).  accepted[s]: drafts that hold; next[s]: the token after
 // them, -1 where a deciding row has NaN or +infinity or nothing but -infinity (a logit of -infinity alone is a token of probability 0), or
-// where lens[s] < 1 or rows are not there.
+// where lens[s] < 1, rows are not there, or are another sequence's too.
 int64_t sp_verify_workspace_floats(int rows, int sequences, int vocab);
 int sp_verify_drafts(void* stream, int dtype, const void* logits, int rows, int vocab, const int32_t* tokens, const int32_t* starts,
                      const int32_t* lens, int sequences, const float* uniform, const float* temperature, const void* draft_logits, int drafted,

@@ -599,6 +599,9 @@ class Q4Matrix:
     """Weights of 4 bits as `gemm_q4` reads them: w[n, k] = (code - 8) * scale[n, k // group].  Made by `q4_pack`."""
 
     def __init__(self, rows: int, cols: int, group: int, words: torch.Tensor, scales: torch.Tensor):
+        groups = _q4_sizes(rows, cols, group)
+        if words.dtype != torch.int32 or words.numel() != library().sp_q4_words(rows, cols) or tuple(scales.shape) != (groups, (rows + 15) // 16 * 16):
+            raise KernelError(f"4-bit weights [{rows}, {cols}] in groups of {group}: words {tuple(words.shape)} and scales {tuple(scales.shape)} do not fit")
         self.rows, self.cols, self.group, self.words, self.scales = rows, cols, group, words, scales
 
     def nbytes(self) -> int:
@@ -651,7 +654,8 @@ def gemm_q4_workspace_floats(dtype: torch.dtype, T: int, N: int, K: int) -> int:
 
 def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False, workspace=None) -> None:
     """out = a @ w.T (+ bias) of a's dtype (float32 or bfloat16); with accumulate, out (float32) += a @ w.T (+ bias).  Made for few tokens: the
-    weights are read once for every 64.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new
+    weights are read once for every 64.  bfloat16 numbers of `a` are multiplied by up to 31 and the excess taken off: beyond some 1e37, and
+    for an infinity, a token's row is NaN.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new
     one, where the product needs any); calls that may run at the same time need one each."""
     stream = _here("gemm_q4", a, w.words, w.scales, out, bias)
     if a.dim() != 2 or a.shape[1] != w.cols or tuple(out.shape) != (a.shape[0], w.rows):
@@ -1706,7 +1710,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, starts: torch.Tens
     max(p - q, 0) of the first that does not, from p of the last row where all do, as the lowest index whose running sum exceeds
     uniform[last row] times the whole; so the tokens are distributed as p has them.  Where the temperature is 0 (or absent) a draft
     holds while it is the lowest index of the maximum, and the next token is that index.  A logit of -infinity is a token that is not
-    allowed; a deciding row with NaN or +infinity, or without any token allowed, gives next_token -1, as `sample` does.
+    allowed; a deciding row with NaN or +infinity, or without any token allowed, gives next_token -1, as `sample` does; so does a
+    sequence whose rows are not among the 1 .. 32767 of `logits`, or are another's too.
     starts, lens: int32, one a sequence; uniform: float32 in [0, 1), one a row; temperature: float32, one a sequence; accepted, next_token: int32."""
     stream = _here("verify_drafts", logits, tokens, starts, lens, uniform, accepted, next_token, workspace, temperature, draft_logits, draft_rows)
     code = _code(logits, "logits")

@@ -53,6 +53,39 @@ def test_against_the_definition(T, N, K, group, dtype):
     assert ((got - want).abs() <= allowed(x, scales, w, group, dtype, want)).all()
 
 
+# Sizes at which other ways are taken: two and four tiles a wave, K in parts, x through LDS with two to four tiles of tokens, and the same without whole eights of K
+WAYS = [(1, 16400, 64, 32), (4, 16390, 136, 64), (16, 7000, 256, 64), (3, 48, 9000, 128), (40, 100, 8200, 32), (17, 4000, 4304, 64), (17, 4000, 4300, 64), (33, 4001, 4304, 128),
+        (64, 4000, 4304, 32), (40, 16390, 1040, 128), (60, 16400, 1040, 32), (1, 16400, 1040, 64), (5, 4000, 4304, 32), (80, 16400, 1040, 64)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("T,N,K,group", WAYS)
+def test_every_way(T, N, K, group, dtype):
+    codes, scales, w = weights(N, K, group, seed=T + N, scale_dtype=F32 if T % 2 else BF16)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(K)).to(dtype)
+    want = x.double() @ w.t()
+    got = product(x, codes, scales, group, K)
+    assert ((got - want).abs() <= allowed(x, scales, w, group, dtype, want)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_tensors_that_start_anywhere(dtype):
+    """x, the result and the workspace at addresses that no 16-byte access takes."""
+    from sprout_lm_amd import ops
+    T, N, K, group = 20, 48, 9000, 128
+    codes, scales, w = weights(N, K, group, seed=3)
+    matrix = ops.q4_pack(codes.to(DEV), scales.to(DEV), group)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(3)).to(dtype)
+    flat = torch.zeros(T * K + 1, dtype=dtype, device=DEV)
+    flat[1:] = x.to(DEV).reshape(-1)
+    room = torch.full((T * N + 2,), 7, dtype=dtype, device=DEV)
+    need = ops.gemm_q4_workspace_floats(dtype, T, N, K)
+    ops.gemm_q4(flat[1:].view(T, K), matrix, room[1:-1].view(T, N), workspace=lambda n: torch.zeros(n + 1, device=DEV)[1:])
+    want = x.double() @ w.t()
+    assert need > 0 and room[0] == 7 and room[-1] == 7
+    assert ((room[1:-1].view(T, N).double().cpu() - want).abs() <= allowed(x, scales, w, group, dtype, want)).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("bias_dtype", [BF16, F32], ids=["bias16", "bias32"])
 def test_bias_and_sums(dtype, bias_dtype):

@@ -66,3 +66,29 @@ def test_tensors_must_be_on_the_gpu():
 def test_a_batch_knows_its_first_query():
     assert ops.AttentionBatch.build([1, 3, 0], [101, 104, 7], "cpu").first_query == 100
     assert ops.AttentionBatch.build([0], [7], "cpu").first_query is None
+
+
+def test_random_numbers_of_a_sequence_are_its_own():
+    from sprout_lm_amd.sampling.sampler import uniform_numbers
+    both = uniform_numbers([5, 2 ** 63 - 1], [0, 7], [400, 600])
+    assert both.dtype == torch.float32 and both.shape == (1000,) and 0 <= float(both.min()) and float(both.max()) < 1
+    assert torch.equal(uniform_numbers([2 ** 63 - 1], [7], [600]), both[400:])
+    assert not torch.equal(uniform_numbers([5], [1], [400]), both[:400]) and not torch.equal(uniform_numbers([6], [0], [400]), both[:400])
+    assert uniform_numbers([], [], []).shape == (0,)
+    assert abs(float(uniform_numbers(list(range(100)), [3] * 100, [100] * 100).double().mean()) - 0.5) < 5 * (1 / 12 / 10000) ** 0.5
+
+
+def test_the_sampler_refuses_rows_that_do_not_fit():
+    from sprout_lm_amd.sampling import Sampler, SamplingParams
+    sampler, one = Sampler(torch.device("cpu"), 5), [SamplingParams()]
+    for logits, tokens, lens, params, counters in ((3, 2, [2], one, [0]), (2, 3, [2], one, [0]), (2, 2, [2, 0], one * 2, [0, 0]), (2, 2, [2], one * 2, [0]), (2, 2, [2], one, [])):
+        with pytest.raises(ValueError, match="verify"):
+            sampler.verify(torch.zeros(logits, 5), torch.zeros(tokens, dtype=torch.int32), lens, params, counters)
+
+
+def test_4_bit_weights_know_their_sizes():
+    words, scales = torch.zeros(2 * 2 * 256, dtype=torch.int32), torch.zeros(5, 32)
+    assert ops.Q4Matrix(20, 130, 32, words, scales).nbytes() == 4096 + 640
+    for args in ((20, 130, 16, words, scales), (33, 130, 32, words, scales), (20, 257, 32, words, scales), (20, 130, 64, words, scales), (20, 130, 32, words.float(), scales)):
+        with pytest.raises(ops.KernelError):
+            ops.Q4Matrix(*args)
