@@ -8,18 +8,18 @@
 // instruction and its shift.  The 24 too much is taken off by the matrix cores: x times rows of -24 is the same for all rows of
 // weights and costs one product beside those of a wave's 16 NT rows.  So the codes, which are whole numbers, meet x unrounded; the sums of a
 // group are float32 and multiplied by the scale in float32.
-// float32 x is taken as the sum of three bfloat16 numbers, which holds all its bits: three products each.  There the codes become code - 8
-// before the product (28 instructions for eight codes instead of 8): sums of numbers five times as large lost as much of the last places.
+// float32 x is taken as the sum of three bfloat16 numbers, which holds all its bits: three products each.  There the codes become
+// (code - 8) / 16 before the product (14 instructions for eight codes instead of 8): sums of numbers five times as large lost as much of the last places.
 //
 // Two kernels.  For a few tokens (gemm_q4.hip) a wave reads its operands of x itself.  A load of them touches 16 rows, which the caches
 // serve at a quarter of their rate: with 64 tokens that took four times as long as everything else.  With more tokens (gemm_q4_staged.h) x comes
 // through LDS, once for the four waves of a block.  Where rows of weights alone do not fill the chip several blocks (`splits`)
 // share out K and a second launch joins them, in a fixed order.
 //
-// One token of bfloat16 by 37,888 x 3,584 in groups of 64: 15.3 us, 4.6 TB/s of weights and scales, near what a copy reaches.  64 tokens by
-// 55,296 x 5,120 in groups of 32: 93 us, 390 TFLOP/s, bound by the vector unit: a group of 32 along K of one row and 16 tokens costs one
-// matrix instruction of 16 cycles, four float32 multiply-adds by the scale, 16 cycles, and of unpacking codes and scales 11 more
-// (in groups of 128: 67 us).  40 tokens of float32 by 3,584 x 18,944: 45 us, three products of bfloat16 each, 118 TFLOP/s of float32.
+// One token of bfloat16 by 37,888 x 3,584 in groups of 64: 15.8 us, 4.4 TB/s of weights and scales, near what a copy reaches.  64 tokens by
+// 55,296 x 5,120 in groups of 32: 85 us, 426 TFLOP/s, bound by the vector unit: a group of 32 along K of 16 rows and 16 tokens costs one
+// matrix instruction of 16 cycles, four float32 multiply-adds by the scale, 16 cycles, and of unpacking codes and scales 11 more (in groups
+// of 128: 66 us).  40 tokens of float32 by 3,584 x 18,944: 36.9 us, three products of bfloat16 each, 147 TFLOP/s of float32.
 #pragma once
 #include "mfma.h"
 #include "sprout_hip.h"
@@ -31,6 +31,7 @@ template <> __device__ __forceinline__ uint16_t from_float<uint16_t>(float f) { 
 
 namespace q4 {
 
+constexpr int kStagedRowTiles = 2;      // tiles of 16 rows of a wave where x comes through LDS
 constexpr int kBlockK = 128;      // k of one 16-byte load of a lane: four steps of 32
 
 struct Q4Args {
@@ -50,14 +51,15 @@ __device__ __forceinline__ uint4 codes_plus_16(uint32_t w) {
   asm("" : "+v"(sixteen));
   return make_uint4(((w << 3) & kMask) | sixteen, ((w >> 1) & kMask) | sixteen, ((w >> 5) & kMask) | sixteen, ((w >> 9) & kMask) | sixteen);
 }
-__device__ __forceinline__ uint32_t less_24(uint32_t pair) {      // (whole numbers up to 8: nothing is lost in the upper halves)
-  const float lo = __uint_as_float(pair << 16) - 24.f, hi = __uint_as_float(pair & 0xffff0000u) - 24.f;
-  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
 __device__ __forceinline__ bf16x8 weights_operand(uint32_t w, uint16_t) { return as_bf16x8(codes_plus_16(w)); }
+// For float32: (code - 8) / 16, exactly, by the conversion of four-bit numbers with a sign; two upper halves make a pair.
+constexpr float kWeightsUnit = 16.f;
+__device__ __forceinline__ uint32_t two_codes(uint32_t first, uint32_t second) {
+  return __builtin_amdgcn_perm(__float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(int(second))), __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(int(first))), 0x07060302u);
+}
 __device__ __forceinline__ bf16x8 weights_operand(uint32_t w, float) {
-  const uint4 c = codes_plus_16(w);
-  return as_bf16x8(make_uint4(less_24(c.x), less_24(c.y), less_24(c.z), less_24(c.w)));
+  const uint32_t t = w ^ 0x88888888u, u = t >> 4;
+  return as_bf16x8(make_uint4(two_codes(t, t >> 16), two_codes(u, u >> 16), two_codes((t >> 8) & 255u, t >> 24), two_codes((u >> 8) & 255u, u >> 24)));
 }
 
 // Scales of a lane's four rows as they lie in memory (S: bfloat16 bits or float32), and their values.
@@ -71,12 +73,19 @@ __device__ __forceinline__ float4 scale_values(const ScaleBits<uint16_t>& b) {
 }
 __device__ __forceinline__ float4 scale_values(const ScaleBits<float>& b) { return b.v; }
 
-// Eight numbers of a token from k on as they lie in memory, zeros behind K, and as operands.  VEC: rows start at whole 16 bytes and K is whole eights.
+// Words asked for earlier have come here, and not been asked for later: a load whose only use lies in a loop's next turn is otherwise
+// moved there, to where it is waited for.
+__device__ __forceinline__ void arrived(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+__device__ __forceinline__ void arrived(ScaleBits<uint16_t>& b) { asm volatile("" : "+v"(b.v.x), "+v"(b.v.y)); }
+__device__ __forceinline__ void arrived(ScaleBits<float>& b) { asm volatile("" : "+v"(b.v.x), "+v"(b.v.y), "+v"(b.v.z), "+v"(b.v.w)); }
+
+// Eight numbers of a token from k on as they lie in memory, and as operands.  VEC: rows start at whole 16 bytes and K is whole eights; behind K
+// the row's first eight are read (a load under a condition is waited for where the condition ends) and cleared before use.  Otherwise zeros lie behind K.
 struct RawBf16 { uint4 v; };
 struct RawF32 { float4 a, b; };
 template <bool VEC> __device__ __forceinline__ void x_load(const uint16_t* row, int k, int K, RawBf16& r) {
   if (VEC) {
-    r.v = k < K ? ldg128(row + k) : make_uint4(0, 0, 0, 0);
+    r.v = ldg128(row + (k < K ? k : 0));
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -86,8 +95,9 @@ template <bool VEC> __device__ __forceinline__ void x_load(const uint16_t* row, 
 }
 template <bool VEC> __device__ __forceinline__ void x_load(const float* row, int k, int K, RawF32& r) {
   if (VEC) {
-    r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (k < K) { r.a = *reinterpret_cast<const float4*>(row + k); r.b = *reinterpret_cast<const float4*>(row + k + 4); }
+    const float* p = row + (k < K ? k : 0);
+    r.a = *reinterpret_cast<const float4*>(p);
+    r.b = *reinterpret_cast<const float4*>(p + 4);
   } else {
     float f[8];
 #pragma unroll
@@ -106,6 +116,8 @@ __device__ __forceinline__ void x_operands(const RawF32& r, bf16x8 (&p)[3]) {
 #pragma unroll
   for (int i = 0; i < 3; ++i) p[i] = as_bf16x8(q[i]);
 }
+__device__ __forceinline__ void clear(RawBf16& r) { r.v = make_uint4(0, 0, 0, 0); }
+__device__ __forceinline__ void clear(RawF32& r) { r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f); }
 template <typename X> struct RawOf;
 template <> struct RawOf<uint16_t> { typedef RawBf16 type; };
 template <> struct RawOf<float> { typedef RawF32 type; };
@@ -134,12 +146,12 @@ template <typename X> __device__ __forceinline__ void store_four(const Q4Args& a
   }
 }
 
-// The plan: row_tiles (of 16 rows a wave), token_tiles (of 16 tokens a block), staged: which kernel.
+// The plan: which kernel, row_tiles (of 16 rows a wave), token_tiles (of 16 tokens a block).
 struct Q4Plan { int row_tiles, token_tiles, splits, staged; };
 
 }  // namespace q4
 
-void gemm_q4_staged_bf16(hipStream_t s, const q4::Q4Args& a, const q4::Q4Plan& p, int steps, int scales_bf16);
-void gemm_q4_staged_f32(hipStream_t s, const q4::Q4Args& a, const q4::Q4Plan& p, int steps, int scales_bf16);
+bool gemm_q4_staged_bf16(hipStream_t s, const q4::Q4Args& a, int token_tiles, int steps, int scales_bf16);
+bool gemm_q4_staged_f32(hipStream_t s, const q4::Q4Args& a, int token_tiles, int steps, int scales_bf16);
 
 }  // namespace sprout

@@ -61,6 +61,7 @@ __global__ __launch_bounds__(256) void gemm_q4_kernel(Q4Args a) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       bf16x8 b[PARTS];
+      if (VEC && 128 * kb + 128 > a.K && 128 * kb + 32 * s + 8 * lj >= a.K) clear(raw[s]);
       x_operands(raw[s], b);
       if (!kF32) off = mfma16(minus24, b[0], s % STEPS == 0 ? zero : off);
 #pragma unroll
@@ -85,6 +86,10 @@ __global__ __launch_bounds__(256) void gemm_q4_kernel(Q4Args a) {
         load_scales(kb_next, s / STEPS);
       }
     }
+  }
+  if (kF32) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) total[n] *= kWeightsUnit;
   }
   if (wave > 0) {
 #pragma unroll
@@ -155,18 +160,18 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const W* __restrict__ 
 }
 
 // Which kernel, how many tiles of 16 rows and tokens a wave or block takes, and over how many blocks K is split (bfloat16 unless float32 is
-// named; us, groups of 128 where nothing else stands; sizes as rows x K).
-//  - x through LDS costs barriers and pays where x is read often and the weights are many: 55,296 x 5,120, 64 tokens of group 32, 85.8
-//    against more than 150; 3,584 x 18,944, 40 tokens of group 64, 29.9 against 33.0; float32 37,888 x 3,584 of group 64, one token, 29.4
-//    against 36.9.  Up to 16 tokens (16 of 37,888 x 3,584: 21.8 without it, 22.8 with) and where 16 Mi weights or fewer are spread over few
-//    blocks (33 tokens of 9,728 x 896: 7.9 against 10.8) it is left out.
+// named; us, groups of 64 where nothing else stands; sizes as rows x K).
+//  - x through LDS costs barriers and pays where x is read often and the weights are many: 3,584 x 18,944, 40 tokens 27.3 against
+//    33.0; float32 37,888 x 3,584, 16 tokens 30.8 against 36.9, one token 27.2 against 31.4.  It is left out up to 16 tokens of bfloat16
+//    (16 of 37,888 x 3,584: 22.7, and 22.8 with it), up to four of float32 on fewer rows (four of 3,584 x 18,944: 23.4, 23.2 with it),
+//    and where 16 Mi weights or fewer are spread over few blocks (33 tokens of 9,728 x 896: 7.9 against 10.8).
 //  - Without it, more tiles a wave read x less often, fewer keep more blocks in flight: one token of 37,888 rows 17.6 with two tiles, 18.8
-//    with four, 21.9 with one; 16 tokens 21.8 with four, 27.3 with two; 3,584 x 3,584 7.1 with one, 7.8 with two.  A long K is better split
+//    with four, 21.9 with one; 16 tokens 22.7 with four, 27.6 with two; 3,584 x 3,584 7.1 with one, 7.8 with two.  A long K is better split
 //    over blocks of four tiles (16 tokens of 3,584 x 18,944: 18.8, two tiles 22.6), a short one over blocks of one tile (one token
 //    of 896 x 4,864: 6.5 in four parts, 7.1 in one; in eight 7.3).
-//  - With it, a wave's two tiles of rows become four where the rows are many (64 tokens of 55,296: 67.3 against 74.2) and 48 or 64 tokens
-//    share a pass; float32's three parts leave room for 32 tokens (64 tokens of 37,888 x 3,584: 82.7, by 16 each 90.8; 40 tokens
-//    leave half of the second 32 empty: 71.1 by 16, 79.6 by 32).  K is split until each compute unit has two blocks (five of float32).
+//  - With it, as many tokens share a block as registers and LDS allow, 64 of bfloat16 (64 of 55,296 x 5,120: 65.6 in groups of 128, by 32 each
+//    71.1) and 48 of float32, whose parts take three times the room (40 of 3,584 x 18,944: 38.9, by 16 each 43.7).  K is split until each
+//    compute unit has two blocks (five of float32: 40 tokens of 37,888 x 3,584 60.8 in four parts, 70.3 in two).
 Q4Plan q4_plan(int x_dtype, int T, int N, int K) {
   Q4Plan p;
   const bool f32 = x_dtype == kF32, small = int64_t(N) * K <= 16 << 20;
@@ -174,9 +179,9 @@ Q4Plan q4_plan(int x_dtype, int T, int N, int K) {
   p.staged = small ? T > 48 : f32 ? T > 4 || tiles >= 1024 : T > 16;
   p.splits = 1;
   if (p.staged) {
-    const int rounds = (tokens + 3) / 4;
-    p.token_tiles = f32 ? (tokens % 2 == 0 ? 2 : 1) : (tokens + rounds - 1) / rounds;
-    p.row_tiles = !f32 && p.token_tiles >= 3 && tiles >= 1024 ? 4 : 2;
+    const int most = f32 ? 3 : 4, rounds = (tokens + most - 1) / most;
+    p.token_tiles = (tokens + rounds - 1) / rounds;
+    p.row_tiles = kStagedRowTiles;
     const int64_t grid = int64_t(tiles + 4 * p.row_tiles - 1) / (4 * p.row_tiles) * ((tokens + p.token_tiles - 1) / p.token_tiles);
     while (grid * p.splits * 4 < (f32 ? 1280 : 448) * 3 && p.splits < 16 && blocks >= 2 * p.splits) p.splits *= 2;
   } else {
@@ -196,14 +201,15 @@ template <typename X, typename S, int NT, bool VEC> void launch_q4_steps(hipStre
   else if (steps == 2) gemm_q4_kernel<X, S, NT, 2, VEC><<<grid, 256, 0, s>>>(a);
   else gemm_q4_kernel<X, S, NT, 4, VEC><<<grid, 256, 0, s>>>(a);
 }
-template <typename X, typename S> void launch_q4_of(hipStream_t s, const Q4Args& a, const Q4Plan& p, int steps, bool vec) {
+template <typename X, typename S> bool launch_q4_of(hipStream_t s, const Q4Args& a, const Q4Plan& p, int steps, bool vec) {
+  bool launched = true;
   if (!vec) launch_q4_steps<X, S, 1, false>(s, a, steps);
-  else if (p.staged && sizeof(X) == 4) gemm_q4_staged_f32(s, a, p, steps, sizeof(S) == 2);
-  else if (p.staged) gemm_q4_staged_bf16(s, a, p, steps, sizeof(S) == 2);
+  else if (p.staged) launched = sizeof(X) == 4 ? gemm_q4_staged_f32(s, a, p.token_tiles, steps, sizeof(S) == 2) : gemm_q4_staged_bf16(s, a, p.token_tiles, steps, sizeof(S) == 2);
   else if (p.row_tiles == 1) launch_q4_steps<X, S, 1, true>(s, a, steps);
   else if (p.row_tiles == 2) launch_q4_steps<X, S, 2, true>(s, a, steps);
   else launch_q4_steps<X, S, 4, true>(s, a, steps);
-  if (a.splits > 1) gemm_q4_join_kernel<X><<<unsigned((size_t(a.T) * a.N + 255) / 256), 256, 0, s>>>(a);
+  if (launched && a.splits > 1) gemm_q4_join_kernel<X><<<unsigned((size_t(a.T) * a.N + 255) / 256), 256, 0, s>>>(a);
+  return launched;
 }
 
 constexpr size_t kMostBlocks = (size_t(1) << 24) - 1;      // a launch has less than 2^32 threads
@@ -281,9 +287,7 @@ extern "C" int sp_gemm_q4(void* stream, int x_dtype, const void* x, const void* 
   const bool vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   hipStream_t s = (hipStream_t)stream;
   const int steps = group / 32;
-  if (x_dtype == kF32 && scale_dtype == kF32) launch_q4_of<float, float>(s, a, p, steps, vec);
-  else if (x_dtype == kF32) launch_q4_of<float, uint16_t>(s, a, p, steps, vec);
-  else if (scale_dtype == kF32) launch_q4_of<uint16_t, float>(s, a, p, steps, vec);
-  else launch_q4_of<uint16_t, uint16_t>(s, a, p, steps, vec);
-  return check_launch("sp_gemm_q4");
+  const bool launched = x_dtype == kF32 ? (scale_dtype == kF32 ? launch_q4_of<float, float>(s, a, p, steps, vec) : launch_q4_of<float, uint16_t>(s, a, p, steps, vec))
+                                        : (scale_dtype == kF32 ? launch_q4_of<uint16_t, float>(s, a, p, steps, vec) : launch_q4_of<uint16_t, uint16_t>(s, a, p, steps, vec));
+  return launched ? check_launch("sp_gemm_q4") : 1;
 }

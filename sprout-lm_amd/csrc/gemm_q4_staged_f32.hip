@@ -5,16 +5,16 @@ namespace sprout {
 
 namespace {
 
-template <typename S> void launch_rows(hipStream_t s, const Q4Args& a, const Q4Plan& p, int steps) {
-  if (p.token_tiles == 1) launch_staged<float, S, 2, 1>(s, a, steps);
-  else launch_staged<float, S, 2, 2>(s, a, steps);
+template <typename S> bool launch_tiles(hipStream_t s, const Q4Args& a, int token_tiles, int steps) {
+  if (token_tiles == 1) return launch_staged<float, S, 1>(s, a, steps);
+  if (token_tiles == 2) return launch_staged<float, S, 2>(s, a, steps);
+  return launch_staged<float, S, 3>(s, a, steps);
 }
 
 }  // namespace
 
-void gemm_q4_staged_f32(hipStream_t s, const Q4Args& a, const Q4Plan& p, int steps, int scales_bf16) {
-  if (scales_bf16) launch_rows<uint16_t>(s, a, p, steps);
-  else launch_rows<float>(s, a, p, steps);
+bool gemm_q4_staged_f32(hipStream_t s, const Q4Args& a, int token_tiles, int steps, int scales_bf16) {
+  return scales_bf16 ? launch_tiles<uint16_t>(s, a, token_tiles, steps) : launch_tiles<float>(s, a, token_tiles, steps);
 }
 
 }  // namespace sprout
