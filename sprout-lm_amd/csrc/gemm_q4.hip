@@ -166,9 +166,9 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const W* __restrict__ 
 //    (16 of 37,888 x 3,584: 22.7, and 22.8 with it), up to four of float32 on fewer rows (four of 3,584 x 18,944: 23.4, 23.2 with it),
 //    and where 16 Mi weights or fewer are spread over few blocks (33 tokens of 9,728 x 896: 7.9 against 10.8).
 //  - Without it, more tiles a wave read x less often, fewer keep more blocks in flight: one token of 37,888 rows 17.6 with two tiles, 18.8
-//    with four, 21.9 with one; 16 tokens 22.7 with four, 27.6 with two; 3,584 x 3,584 7.1 with one, 7.8 with two.  A long K is better split
-//    over blocks of four tiles (16 tokens of 3,584 x 18,944: 18.8, two tiles 22.6), a short one over blocks of one tile (one token
-//    of 896 x 4,864: 6.5 in four parts, 7.1 in one; in eight 7.3).
+//    with four, 21.9 with one; 16 tokens 22.7 with four, 27.6 with two; 3,584 x 3,584 7.1 with one, 7.8 with two.  A long K of few rows
+//    is better split over blocks of four tiles (16 tokens of 3,584 x 18,944: 18.8, two tiles 22.6; one tile, not split, 28.0); splitting a short
+//    one gains less than a second launch costs the host (one token of 896 x 4,864: 7.1, in four parts 6.5, called one by one 8 and 11.8).
 //  - With it, as many tokens share a block as registers and LDS allow, 64 of bfloat16 (64 of 55,296 x 5,120: 65.6 in groups of 128, by 32 each
 //    71.1) and 48 of float32, whose parts take three times the room (40 of 3,584 x 18,944: 38.9, by 16 each 43.7).  K is split until each
 //    compute unit has two blocks (five of float32: 40 tokens of 37,888 x 3,584 60.8 in four parts, 70.3 in two).
@@ -190,7 +190,7 @@ Q4Plan q4_plan(int x_dtype, int T, int N, int K) {
     p.token_tiles = 1;
     p.row_tiles = long_k ? 4 : T <= 4 ? (units >= 1024 ? 2 : 1) : units >= 600 ? 4 : units >= 400 ? 2 : 1;
     const int64_t grid = int64_t(tiles + p.row_tiles - 1) / p.row_tiles * tokens;
-    while (grid * p.splits * 2 <= (long_k ? 512 : 256) && blocks >= 2 * p.splits * (long_k ? 16 : 8)) p.splits *= 2;
+    while (long_k && grid * p.splits * 2 <= 512 && blocks >= 32 * p.splits) p.splits *= 2;
   }
   return p;
 }
