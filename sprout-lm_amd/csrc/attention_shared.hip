@@ -15,6 +15,12 @@
 // instruction takes them; nothing is rounded before the result.  Values lie in LDS as the second product reads them, runs of two pieces
 // of 16 bytes a dimension: 1 KB a read and 1 KB a load, whose lanes' addresses are one number a lane beside scalars.
 // Weights are rounded to bfloat16 for the product with the values (half a step each); the sum of the weights is of the unrounded ones.
+//
+// Heads of 128, bfloat16: 16 sequences of one query behind 32,000 keys (40 heads in 8 groups) 44.8 us, 3.3 TB/s; 64 of 1 to 5 queries behind
+// 8,192 keys and 64 to 1,024 own (28 heads in 4 groups) 54.5 us, 436 TFLOP/s.  Neither bytes nor products bound these: a stage of 64 keys by
+// 128 rows takes a CU 1.35 us, of which the matrix cores work 0.43 and the vector unit as long, one after the other in a wave, and two
+// blocks on a CU take more than twice as long as one; a sixth is the loads.  Small batches are bound by two launches and the trips from table to page to
+// product: four sequences behind 500 keys 8.8 + 4.1 us.
 #include <type_traits>
 
 #include "mfma.h"
@@ -540,32 +546,37 @@ int keys_of_stage(int dtype, int held) {
 struct SharedPlan { int prefix_splits, prefix_keys, row_blocks, block_rows, own_splits, own_keys, own_rows; };
 
 // How the work is cut: the shared keys of a block of rows into the number of parts with the least estimated time in microseconds.  A
-// stage takes 1.35 while a CU has one block, twice that with two (their products, exponentials and LDS reads hardly overlap), and every
-// further block waits; a block's start and end are the same for all; a part costs the joining launch what it writes and reads again.  Own keys
-// are cut where a block would have more stages than one of the shared keys, and four at least: most sequences' are fewer, and a block without
-// keys still costs its start.  (64 sequences of 1 to 5 queries of 28 heads of 128 behind 8,192 keys, products of the own keys left out:
-// 1, 5, 6, 9, 11 parts 189, 57, 52, 42, 47 us and 6, 7, 7, 15, 15 to join them.)
+// stage takes 1.35 alone on the chip and 0.85 more for every block that an XCD's CUs have on average (2.2 with one, 3.0 with two: measured with 44 to
+// 484 blocks); units of a part and a key/value head go round the XCDs whole, so an XCD has the rows' blocks of some or of one unit more; behind two
+// blocks a CU the rest waits.  A part costs what it writes and the joining launch reads.  A block of own keys counts for a quarter, as few rows share
+// its waves' work.  Own keys come last and are cut into half as many stages, so that the end is even, and four at least; of float32, whose stages
+// take four times as long, one (8 sequences of 3 queries behind 1,500 keys and 8 to 200 own: 15.8 us, with four 21.1).
+// (64 sequences of 1 to 5 queries of 28 heads of 128 behind 8,192 keys, in all: 5, 7, 8, 9, 10, 11 parts 64.5, 57.5, 56.4, 62.4, 62.1, 65.0 us; 16 of
+// one query of 40 heads behind 32,000: 25, 32, 48, 64 parts 43.2, 39.5, 38.2, 43.0.)
 SharedPlan shared_plan(int dtype, int hd, int nq, int nkv, int tokens, int n_tiles, int prefix, int max_own) {
   SharedPlan p;
   const int G = nq / nkv, held = held_dims(hd), stage = keys_of_stage(dtype, held), rows = tokens * G;
   p.row_blocks = (rows + 127) / 128;
   p.block_rows = ((rows + p.row_blocks - 1) / p.row_blocks + 31) / 32 * 32;
   p.row_blocks = (rows + p.block_rows - 1) / p.block_rows;
-  const int stages = (prefix + stage - 1) / stage, walks = p.row_blocks * nkv;
+  const int stages = (prefix + stage - 1) / stage;
   const int most = tokens - (n_tiles - 1) < kSharedTile ? tokens - (n_tiles - 1) : kSharedTile;      // every entry has a query
   p.own_rows = (most * G + 127) / 128;
-  const double own_blocks = double(n_tiles) * ((tokens + n_tiles - 1) / n_tiles * G + 127) / 128 * nkv, part = double(tokens) * nq * held * 8.0 / 3.0e6;
+  const double own_blocks = double(n_tiles) * ((tokens + n_tiles - 1) / n_tiles * G + 127) / 128 * nkv, part = double(tokens) * nq * held * 8.0 / 1.5e6;
   double best = 1.0e30;
   int chosen = 1;
   for (int splits = 1; splits <= 64 && splits <= stages; ++splits) {
     const int per = (stages + splits - 1) / splits;
-    const double load = (double(splits) * walks + 0.5 * own_blocks) / 256.0;
-    const double time = 1.35 * per * (load > 1.0 ? load : 1.0) + splits * part;
+    const int units = (splits * nkv + 7) / 8;      // of an XCD
+    const double load = (double(units) * p.row_blocks + own_blocks / 32.0) / 32.0;
+    const double time = per * (1.35 + 0.85 * load) * (load > 2.0 ? load / 2.0 : 1.0) + splits * part;
     if (time < best) { best = time; chosen = per; }
   }
   p.prefix_keys = chosen * stage;
   p.prefix_splits = (stages + chosen - 1) / chosen;
-  p.own_keys = (chosen > 4 ? chosen : 4) * stage;
+  const int least = dtype == kF32 ? 1 : 4, own_stages = (max_own + stage - 1) / stage, of_64 = (own_stages + 63) / 64;      // 64 parts at most, as of the shared keys
+  const int own = chosen / 2 > least ? chosen / 2 : least;
+  p.own_keys = (own > of_64 ? own : of_64) * stage;
   p.own_splits = (max_own + p.own_keys - 1) / p.own_keys;
   return p;
 }

@@ -11,12 +11,13 @@
 // errors here (2e-10 of a weight that is compared or drawn from, 1e-9 of a row's sum) move an answer once in millions of draws; float32
 // sums would once in a thousand.  Reading the rows' logits bounds the whole.  So that it takes longer than weighing them, sums use a
 // table and a float32 polynomial, single weights a float64 polynomial of degree 8 (the library's exponential took 184 us of 646 rows
-// of 152,064, the float64 polynomial 110, this 76).
+// of 152,064, the float64 polynomial 110, this 70 to 76).
 //
 // Four launches: maximum and sum of every row by chunks, so that few rows fill the chip as many do; a block per sequence, a wave a row,
 // joins them and finds the deciding row; a block per chunk and sequence sums what is left there; a block per sequence finds chunk and token.
-// 64 sequences of up to 7 drafts over 152,064 tokens of bfloat16, 354 MB: 76, 7.3, 20.9 and 11.5 us, 3.0 TB/s over all and 4.6 in the first.
-// (The second and third in one, every block of a sequence deciding by itself: 52 us where the two take 28.)
+// 64 sequences of up to 7 drafts over 152,064 tokens of float32, 354 MB: 70, 7.7, 20.8 and 11.3 us, 3.1 TB/s over all and 5.0 in the first.
+// (The second and third in one, every block of a sequence deciding by itself: 52 us where the two take 28.  The third and fourth in one, a
+// sequence's last block drawing: 148 us where the two take 32, for the fences by which its blocks hand over their sums drop an XCD's L2.)
 #include "common.h"
 #include "sprout_hip.h"
 

@@ -126,6 +126,11 @@ def test_against_the_definition(case, dtype):
     check(Case(dtype, *CASES[case], seed=case))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_own_keys_longer_than_the_shared(dtype):
+    check(Case(dtype, 3, 1, 64, 16, 40, [(1, 9000), (2, 4200), (1, 1)], seed=5))
+
+
 @pytest.mark.parametrize("sequences", [31, 64, 150])
 def test_many_sequences(sequences):
     check(Case(BF16, 14, 2, 64, 16, 300, [(1 + i % 3, 3 + i % 29) for i in range(sequences)], seed=sequences))
