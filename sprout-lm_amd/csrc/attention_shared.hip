@@ -631,7 +631,7 @@ extern "C" int sp_attention_shared(void* stream, int dtype, const void* q, int q
   SP_REQUIRE(dtype == kF32 || dtype == kBF16, "sp_attention_shared: unsupported dtype %d", dtype);
   SP_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "sp_attention_shared: %d query heads do not divide into %d groups", nq, nkv);
   SP_REQUIRE(hd > 0 && hd <= 256, "sp_attention_shared: head size %d is outside 1..256", hd);
-  SP_REQUIRE(page_size > 0 && num_pages > 0 && max_blocks > 0, "sp_attention_shared: bad cache geometry");
+  SP_REQUIRE(page_size > 0 && num_pages > 0 && max_blocks > 0 && int64_t(max_blocks) * page_size < int64_t(1) << 31, "sp_attention_shared: bad cache geometry");
   SP_REQUIRE(n_tiles >= 0 && tokens >= n_tiles, "sp_attention_shared: %d tiles of queries for %d rows", n_tiles, tokens);
   if (n_tiles == 0) return 0;
   SP_REQUIRE(q && k_pool && v_pool && block_tables && q_start && q_len && ctx_len && tiles && out && (prefix_table || prefix == 0),

@@ -272,7 +272,7 @@ extern "C" int sp_gemm_q4(void* stream, int x_dtype, const void* x, const void* 
   if (T == 0) return 0;
   SP_REQUIRE(x && words && scales && out, "sp_gemm_q4: null argument");
   SP_REQUIRE(reinterpret_cast<uintptr_t>(words) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 16 == 0, "sp_gemm_q4: packed weights must start at a multiple of 16 bytes");
-  SP_REQUIRE(T <= 65535 * 16 && K < 1 << 25, "sp_gemm_q4: %d tokens, K=%d", T, K);      // (64 rows of x within 32 bits)
+  SP_REQUIRE(T <= 65535 * 16 && K <= 1 << 24, "sp_gemm_q4: %d tokens, K=%d", T, K);      // (64 rows of x within 32 bits)
   Q4Args a;
   a.x = x; a.words = static_cast<const uint32_t*>(words); a.scales = scales; a.bias = bias; a.out = out;
   a.T = T; a.N = N; a.K = K; a.blocks = (K + kBlockK - 1) / kBlockK; a.groups = (K + group - 1) / group; a.padded = (N + 15) / 16 * 16;

@@ -468,7 +468,7 @@ extern "C" int sp_verify_drafts(void* stream, int dtype, const void* logits, int
                                 int drafted, const int32_t* draft_rows, int32_t* accepted, int32_t* next, void* workspace,
                                 int64_t workspace_floats) {
   SP_REQUIRE(dtype == kF32 || dtype == kBF16, "sp_verify_drafts: unsupported dtype %d", dtype);
-  SP_REQUIRE(rows >= 0 && sequences >= 0 && vocab > 0 && drafted >= 0, "sp_verify_drafts: bad sizes rows=%d sequences=%d vocab=%d drafted=%d", rows, sequences, vocab, drafted);
+  SP_REQUIRE(rows >= 0 && sequences >= 0 && vocab > 0 && vocab <= 1 << 30 && drafted >= 0, "sp_verify_drafts: bad sizes rows=%d sequences=%d vocab=%d drafted=%d", rows, sequences, vocab, drafted);
   if (sequences == 0) return 0;
   SP_REQUIRE(rows > 0 && rows <= 32767, "sp_verify_drafts: %d rows are outside 1..32767", rows);
   SP_REQUIRE(sequences <= 65535, "sp_verify_drafts: %d sequences are more than 65535", sequences);

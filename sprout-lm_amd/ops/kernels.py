@@ -1712,7 +1712,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, starts: torch.Tens
     holds while it is the lowest index of the maximum, and the next token is that index.  A logit of -infinity is a token that is not
     allowed; a deciding row with NaN or +infinity, or without any token allowed, gives next_token -1, as `sample` does; so does a
     sequence whose rows are not among the 1 .. 32767 of `logits`, or are another's too.
-    starts, lens: int32, one a sequence; uniform: float32 in [0, 1), one a row; temperature: float32, one a sequence; accepted, next_token: int32."""
+    starts, lens: int32, one a sequence; uniform: float32 in [0, 1), one a row; temperature: float32, one a sequence (below 0 or NaN: as 0); accepted,
+    next_token: int32; workspace: `verify_workspace_floats`, one for each of the calls that may run at the same time."""
     stream = _here("verify_drafts", logits, tokens, starts, lens, uniform, accepted, next_token, workspace, temperature, draft_logits, draft_rows)
     code = _code(logits, "logits")
     if logits.dim() != 2:

@@ -244,6 +244,12 @@ def test_rows_of_two_sequences(warmth):
     assert following == [wanted[1][0], -1, wanted[1][2], wanted[1][3], -1, -1, -1, -1]
 
 
+@pytest.mark.parametrize("warmth", [-1.0, math.nan])
+def test_temperatures_below_zero_are_greedy(warmth):
+    data = inputs(300, [2, 3], seed=12)
+    assert call(**data, temperature=torch.tensor([warmth, 1.0])) == definition(**data, temperature=torch.tensor([0.0, 1.0]))
+
+
 def test_a_drafter_without_rows():
     data = inputs(90, [3, 2], seed=8, drawn=0.0)
     data["draft_logits"] = torch.zeros(0, 90)

@@ -15,7 +15,7 @@ def test_shared_attention_refuses_at_the_c_interface():
     lib = ops.library()
     #       stream dtype q stride k  v  tables max table prefix start len ctx tiles n max_ctx T ws floats out nq nkv hd page pages scale cap sinks
     good = [None, 1, 16, 256, 16, 16, 16, 9, 16, 100, 16, 16, 16, 16, 2, 110, 2, 16, 1 << 40, 16, 4, 2, 64, 16, 9, 0.1, 0.0, None]
-    for at, value, match in ((1, 2, "dtype"), (20, 3, "divide"), (22, 257, "head size"), (22, 0, "head size"), (23, 0, "geometry"), (7, 0, "geometry"), (16, 1, "rows"), (2, None, "null"),
+    for at, value, match in ((1, 2, "dtype"), (20, 3, "divide"), (22, 257, "head size"), (22, 0, "head size"), (23, 0, "geometry"), (7, 0, "geometry"), (7, 1 << 28, "geometry"), (16, 1, "rows"), (2, None, "null"),
                              (8, None, "null"), (3, 255, "stride"), (9, 110, "fit"), (15, 145, "fit"), (9, -1, "fit"), (26, -1.0, "cap"), (18, 10, "workspace"),
                              (17, None, "workspace")):
         refused(lib.sp_attention_shared, *good[:at], value, *good[at + 1:], match=match)
@@ -28,7 +28,7 @@ def test_drafts_refuse_at_the_c_interface():
     lib = ops.library()
     #       stream dtype logits rows vocab tokens starts lens sequences uniform temperature drafter drafted rows accepted next workspace floats
     good = [None, 0, 16, 4, 50, 16, 16, 16, 2, 16, 16, 16, 3, 16, 16, 16, 16, 1 << 40]
-    for at, value, match in ((1, 2, "dtype"), (3, -1, "sizes"), (4, 0, "sizes"), (3, 0, "rows"), (3, 32768, "rows"), (8, 65536, "sequences"), (2, None, "null"), (9, None, "null"),
+    for at, value, match in ((1, 2, "dtype"), (3, -1, "sizes"), (4, 0, "sizes"), (4, (1 << 30) + 1, "sizes"), (3, 0, "rows"), (3, 32768, "rows"), (8, 65536, "sequences"), (2, None, "null"), (9, None, "null"),
                              (11, None, "together"), (13, None, "together"), (16, None, "workspace"), (16, 4, "workspace"), (17, 3, "workspace")):
         refused(lib.sp_verify_drafts, *good[:at], value, *good[at + 1:], match=match)
     assert lib.sp_verify_drafts(*good[:8], 0, *good[9:]) == 0
@@ -40,7 +40,7 @@ def test_4_bit_products_refuse_at_the_c_interface():
     #       stream dtype x  words dtype scales dtype bias mode dtype out T  N  K  group workspace floats
     good = [None, 1, 16, 16, 1, 16, 0, None, 0, 1, 16, 2, 20, 64, 32, None, 0]
     for at, value, match in ((1, 2, "dtypes"), (4, 2, "dtypes"), (6, 2, "dtypes"), (8, 1, "stores"), (8, 2, "stores"), (9, 0, "stores"), (11, -1, "groups"), (12, 0, "groups"), (13, 0, "groups"),
-                             (14, 16, "groups"), (2, None, "null"), (5, None, "null"), (3, 20, "16 bytes"), (5, 8, "16 bytes"), (11, 1 << 21, "tokens")):
+                             (14, 16, "groups"), (2, None, "null"), (5, None, "null"), (3, 20, "16 bytes"), (5, 8, "16 bytes"), (11, 1 << 21, "tokens"), (13, (1 << 24) + 1, "tokens")):
         refused(lib.sp_gemm_q4, *good[:at], value, *good[at + 1:], match=match)
     assert lib.sp_gemm_q4(*good[:11], 0, *good[12:]) == 0
     refused(lib.sp_q4_pack, None, 16, 2, 16, 20, 64, 32, 16, 16, match="dtype")
