@@ -15,9 +15,10 @@
 //
 // Four launches: maximum and sum of every row by chunks, so that few rows fill the chip as many do; a block per sequence, a wave a row,
 // joins them and finds the deciding row; a block per chunk and sequence sums what is left there; a block per sequence finds chunk and token.
+// For few sequences the third launch does the second's work too (kDecidingBlocks).
 // 64 sequences of up to 7 drafts over 152,064 tokens of float32, 354 MB: 70, 7.7, 20.8 and 11.3 us, 3.1 TB/s over all and 5.0 in the first.
-// (The second and third in one, every block of a sequence deciding by itself: 52 us where the two take 28.  The third and fourth in one, a
-// sequence's last block drawing: 148 us where the two take 32, for the fences by which its blocks hand over their sums drop an XCD's L2.)
+// (The third and fourth in one, a sequence's last block drawing: 148 us where the two take 32, for the fences by which its blocks hand over
+// their sums drop an XCD's L2.)
 #include "common.h"
 #include "sprout_hip.h"
 
@@ -197,20 +198,23 @@ __device__ __forceinline__ RowStat row_stat(const ChunkStat* stats, int chunks, 
   return {wave_sum64(sum), top, bad || !(top > -INFINITY) ? -1 : best};
 }
 
-template <typename T>
-__global__ __launch_bounds__(512) void verify_decide_kernel(VerifyArgs a) {
-  constexpr int kRows = 8;      // rows of a sequence at a time, a wave each; the last row of a sequence never holds
+// A sequence's deciding row, into `found` (shared memory; a barrier follows); `say`: this block writes the answers down.  kRows waves take that
+// many rows at a time; the last row of a sequence never holds.
+template <typename T, int kRows> __device__ __forceinline__ void decide(const VerifyArgs& a, int seq, bool say, Decision& found) {
   __shared__ Decision s_found[kRows];
   __shared__ int s_holds[kRows], s_next[kRows];
-  const int seq = blockIdx.x, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6;
   const int start = a.starts[seq], len = a.lens[seq];
   bool refused = !rows_there(a, start, len);
-  for (int s = threadIdx.x; s < a.sequences; s += 512) {
+  for (int s = threadIdx.x; s < a.sequences; s += 64 * kRows) {
     const int other = a.starts[s], n = a.lens[s];
     if (s != seq && !refused && rows_there(a, other, n) && other < start + len && start < other + n) refused = true;
   }
   if (__syncthreads_or(refused)) {      // rows that are not there, or also another sequence's, whose temperature may differ
-    if (threadIdx.x == 0) { a.accepted[seq] = 0; a.next[seq] = -1; a.decisions[seq].kind = 2; }
+    if (threadIdx.x == 0) {
+      found.kind = 2;
+      if (say) { a.accepted[seq] = 0; a.next[seq] = -1; a.decisions[seq].kind = 2; }
+    }
     return;
   }
   const float temp = temperature_of(a, seq);
@@ -256,14 +260,22 @@ __global__ __launch_bounds__(512) void verify_decide_kernel(VerifyArgs a) {
     while (stop < n && s_holds[stop]) ++stop;
     if (stop < n) {      // (the same in every thread)
       if (threadIdx.x == 0) {
-        a.accepted[seq] = first + stop;
-        a.decisions[seq] = s_found[stop];
-        if (s_found[stop].kind == 2) a.next[seq] = s_next[stop];
+        found = s_found[stop];
+        if (say) {
+          a.accepted[seq] = first + stop;
+          a.decisions[seq] = s_found[stop];
+          if (s_found[stop].kind == 2) a.next[seq] = s_next[stop];
+        }
       }
       return;
     }
     __syncthreads();
   }
+}
+
+template <typename T> __global__ __launch_bounds__(512) void verify_decide_kernel(VerifyArgs a) {
+  __shared__ Decision found;
+  decide<T, 8>(a, blockIdx.x, true, found);
 }
 
 // What is left of a token's probability in the deciding row, of logits p and q (drawn: q from the drafter's row).  kind 0: all of it, else
@@ -275,45 +287,57 @@ __device__ __forceinline__ double left_of(const Decision& d, bool drawn, double 
   return mine > other ? mine - other : 0.0;
 }
 
-// (Loops that are not unrolled over the sixteen: few blocks run these, and code that is run once costs its own way from memory.)
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void verify_left_kernel(VerifyArgs a) {
-  __shared__ double s_sum[4];
+// What is left in a chunk of the deciding row.  DECIDES: every block of a sequence finds that row itself, with twice the waves.  (Loops that are not
+// unrolled over a thread's logits: few blocks run this, and code that is run once costs its own way from memory.)
+template <typename T, bool VEC, bool DECIDES>
+__global__ __launch_bounds__(DECIDES ? 512 : 256) void verify_left_kernel(VerifyArgs a) {
+  constexpr int kThreads = DECIDES ? 512 : 256, kGroups = kVerifyChunk / (4 * kThreads);
+  __shared__ double s_sum[kThreads / 64];
+  __shared__ Decision s_decision;
   const int chunk = blockIdx.x, seq = blockIdx.y, wave = threadIdx.x >> 6;
-  const Decision d = a.decisions[seq];
+  if (DECIDES) {
+    decide<T, kThreads / 64>(a, seq, chunk == 0, s_decision);
+    __syncthreads();
+  }
+  const Decision d = DECIDES ? s_decision : a.decisions[seq];
   if (d.kind == 2) return;
   const bool drawn = d.kind == 1 && d.draft_row >= 0;
   const T* row = static_cast<const T*>(a.logits) + size_t(d.row) * a.vocab;
   const T* draft_row = drawn ? static_cast<const T*>(a.draft_logits) + size_t(d.draft_row) * a.vocab : row;
   const double degree = d.degree;
   float p[4], q[4];
+  auto first_of = [&](int group) { return chunk * kVerifyChunk + 4 * kThreads * group + (VEC ? 4 : 1) * int(threadIdx.x); };
   auto load = [&](int group) __attribute__((always_inline)) {
-    const int i = chunk * kVerifyChunk + 1024 * group + (VEC ? 4 : 1) * int(threadIdx.x);
+    const int i = first_of(group);
     if (VEC) {
       load_four(row, i, a.vocab, p);
       load_four(draft_row, i, a.vocab, q);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        p[j] = i + 256 * j < a.vocab ? to_float(row[i + 256 * j]) : -INFINITY;
-        q[j] = i + 256 * j < a.vocab ? to_float(draft_row[i + 256 * j]) : -INFINITY;
+        p[j] = i + kThreads * j < a.vocab ? to_float(row[i + kThreads * j]) : -INFINITY;
+        q[j] = i + kThreads * j < a.vocab ? to_float(draft_row[i + kThreads * j]) : -INFINITY;
       }
     }
   };
   double sum = 0.0;
   load(0);
 #pragma unroll 1
-  for (int group = 0; group < 4; ++group) {
+  for (int group = 0; group < kGroups; ++group) {
     const float p_now[4] = {p[0], p[1], p[2], p[3]}, q_now[4] = {q[0], q[1], q[2], q[3]};
-    if (group < 3) load(group + 1);
+    if (group + 1 < kGroups) load(group + 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      sum += left_of(d, drawn, degree, p_now[j], q_now[j], chunk * kVerifyChunk + 1024 * group + (VEC ? 4 * int(threadIdx.x) + j : int(threadIdx.x) + 256 * j));
+    for (int j = 0; j < 4; ++j) sum += left_of(d, drawn, degree, p_now[j], q_now[j], first_of(group) + (VEC ? j : kThreads * j));
   }
   sum = wave_sum64(sum);
   if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) a.left[size_t(seq) * a.chunks + chunk] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) all += s_sum[w];
+    a.left[size_t(seq) * a.chunks + chunk] = all;
+  }
 }
 
 constexpr int kDrawThreads = kVerifyChunk / 4;
@@ -443,11 +467,17 @@ size_t verify_bytes(int rows, int sequences, int vocab) {
   return 2 * size_t(rows) * c * sizeof(ChunkStat) + size_t(sequences) * c * sizeof(double) + size_t(sequences) * sizeof(Decision);
 }
 
+// Up to so many blocks of what is left decide by themselves: one launch less, but the same work in every block of a sequence (rows of 151,936: 1,
+// 4, 9, 20 sequences 22.1, 24.3, 32.4, 41.5 us and 24.3, 26.8, 34.6, 43.4 with a launch of its own; 27, 40, 64 sequences 54.9, 70.9, 124 and 52.5, 65.6, 110).
+constexpr int kDecidingBlocks = 768;
+
 template <typename T, bool VEC> int launch_verify(hipStream_t s, const VerifyArgs& a) {
   verify_stats_kernel<T, VEC><<<dim3(a.chunks, a.rows * (a.draft_logits ? 2 : 1)), 256, 0, s>>>(a);
-  verify_decide_kernel<T><<<a.sequences, 512, 0, s>>>(a);
+  const bool few = a.temperature && int64_t(a.chunks) * a.sequences <= kDecidingBlocks;
+  if (!few) verify_decide_kernel<T><<<a.sequences, 512, 0, s>>>(a);
   if (a.temperature) {
-    verify_left_kernel<T, VEC><<<dim3(a.chunks, a.sequences), 256, 0, s>>>(a);
+    if (few) verify_left_kernel<T, VEC, true><<<dim3(a.chunks, a.sequences), 512, 0, s>>>(a);
+    else verify_left_kernel<T, VEC, false><<<dim3(a.chunks, a.sequences), 256, 0, s>>>(a);
     verify_draw_kernel<T, VEC><<<a.sequences, kDrawThreads, 0, s>>>(a);
   }
   return check_launch("sp_verify_drafts");

@@ -110,6 +110,23 @@ def test_many_sequences(sequences):
     assert sequences == 1 or (0 < sum(got[0]) < sum(lens) - sequences)      # some drafts hold, some do not
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [17000, 17001])
+def test_many_sequences_of_many_chunks(vocab, dtype):
+    """So many that decisions are a launch of their own; among them rows that are not there and rows of two sequences."""
+    lens = [1 + i % 5 for i in range(160)]
+    data = inputs(vocab, lens, seed=vocab, dtype=dtype)
+    temperature = torch.tensor([0.0, 1.0, 0.6, 1.3])[torch.arange(160) % 4]
+    check(dict(data, temperature=temperature))
+    rows = len(data["logits"])
+    more = {**data, "starts": data["starts"] + [rows - 1, -4, data["starts"][7]], "lens": lens + [2, 3, 1]}      # the last: the eighth sequence's first row
+    accepted, following = call(**more, temperature=torch.cat([temperature, torch.ones(3)]))
+    wanted = definition(**data, temperature=temperature)
+    keep = [i for i in range(160) if i != 7]
+    assert [accepted[i] for i in keep] == [wanted[0][i] for i in keep] and [following[i] for i in keep] == [wanted[1][i] for i in keep]
+    assert accepted[160:] == [0, 0, 0] and following[160:] == [-1, -1, -1] and (accepted[7], following[7]) == (0, -1)
+
+
 def test_numbers_at_their_ends():
     """The smallest and the largest uniform number; tokens that are not allowed before and behind the only one that is."""
     data = inputs(300, [3, 3, 3, 3], seed=5)
