@@ -96,17 +96,6 @@ __device__ __forceinline__ uint4 weights_of(const floatx16& s, int part, float) 
   return make_uint4(__float_as_uint(s[4 * part]), __float_as_uint(s[4 * part + 1]), __float_as_uint(s[4 * part + 2]), __float_as_uint(s[4 * part + 3]));
 }
 
-// 64 lanes x 16 bytes from base + offset[lane] into LDS at lds_address + 16 lane.
-__device__ __forceinline__ void run_to_lds(uint64_t base, uint32_t offset, uint32_t lds_address) {
-  asm volatile(
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %0, %1"
-      :
-      : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds_address))
-      : "memory", "m0");
-}
-
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 // Keys of a stage, of which two lie in LDS: 32 KB (heads of 256 in float32: 64), at most 128 keys.
 template <typename E, int HD> constexpr int stage_keys() { return HD * int(sizeof(E)) <= 128 ? 128 : HD * int(sizeof(E)) <= 256 ? 64 : 32; }
@@ -223,8 +212,8 @@ __global__ __launch_bounds__(kThreads, HD * sizeof(E) <= 256 ? 2 : 1) void atten
     for (int u = 0; u < LOADS; ++u) {
       if (key0 + (wave + kWaves * u) / DT * GROUP >= hi) break;      // keys behind the last: their values are cleared, their scores masked
       auto start = [&](int from) { return uint64_t(uint32_t(__builtin_amdgcn_readlane(run_high, from))) << 32 | uint32_t(__builtin_amdgcn_readlane(run_low, from)); };
-      if (whole || k_there[u]) run_to_lds(start(u), k_lane[u], at + 1024 * kWaves * u);
-      if (whole || v_there[u]) run_to_lds(start(16 + u), v_lane, at + HALF + 1024 * kWaves * u);
+      if (whole || k_there[u]) lanes_to_lds(start(u), k_lane[u], at + 1024 * kWaves * u);
+      if (whole || v_there[u]) lanes_to_lds(start(16 + u), v_lane, at + HALF + 1024 * kWaves * u);
     }
   };
   // Number by number, a piece at a time.

@@ -15,18 +15,6 @@ using namespace q4;
 
 namespace {
 
-__device__ __forceinline__ void lanes_to_lds(const void* base, uint32_t offset, uint32_t lds_address) {
-  const uint64_t at = reinterpret_cast<uint64_t>(base);
-  const uint64_t scalar = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(at >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(at)));
-  asm volatile(
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %0, %1"
-      :
-      : "v"(offset), "s"(scalar), "s"(__builtin_amdgcn_readfirstlane(lds_address))
-      : "memory", "m0");
-}
-
 // K is whole eights, rows of x start at whole 16 bytes.
 template <typename X, typename S, int TT, int STEPS>
 __global__ __launch_bounds__(256, 2) void gemm_q4_staged_kernel(Q4Args a) {
@@ -68,6 +56,8 @@ __global__ __launch_bounds__(256, 2) void gemm_q4_staged_kernel(Q4Args a) {
   };
   // A wave brings its step of 32 of every token tile; a lane's piece is eight numbers of a token.
   const X* x = static_cast<const X*>(a.x) + size_t(t0) * a.K;
+  const uint64_t x_at = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uint64_t>(x) >> 32)))) << 32 |
+                        uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uint64_t>(x))));
   const int piece_k = 32 * wave + 8 * lj;
   uint32_t piece_at[TT];
 #pragma unroll
@@ -84,7 +74,7 @@ __global__ __launch_bounds__(256, 2) void gemm_q4_staged_kernel(Q4Args a) {
         raw[u].a = *reinterpret_cast<const float4*>(p);
         raw[u].b = *reinterpret_cast<const float4*>(p + 4);
       } else {
-        lanes_to_lds(x, piece_at[u] + in_row, lds_base + buffer * STAGE + 1024 * (wave * TT + u));
+        lanes_to_lds(x_at, piece_at[u] + in_row, lds_base + buffer * STAGE + 1024 * (wave * TT + u));
       }
     }
   };

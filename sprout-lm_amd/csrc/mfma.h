@@ -48,4 +48,17 @@ __device__ __forceinline__ void three_parts(float a, float b, uint32_t& p1, uint
   p3 = pack_bf16x2(a, b);
 }
 
+// 64 lanes x 16 bytes from base + offset[lane] into LDS at lds_address + 16 lane; base and lds_address are the same in all lanes.  A load may
+// read a scalar register five wait states after a vector instruction (a lane read out) wrote it, and the compiler counts none
+// for what an assembly block reads: the move to m0 and s_nop 3 are five.
+__device__ __forceinline__ void lanes_to_lds(uint64_t base, uint32_t offset, uint32_t lds_address) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 3\n\t"
+      "global_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds_address))
+      : "memory", "m0");
+}
+
 }  // namespace sprout
