@@ -331,7 +331,7 @@ def context_from(step: StepArrays, dev: list, n_groups: int, workspace: Workspac
                                        step.max_ctx if max_ctx is None else max_ctx,
                                        step.mean_walk if mean_walk is None else mean_walk,
                                        step.max_tile_ctx if max_tile_ctx is None else max_tile_ctx, step.one_query_keys,
-                                       int(step.host["first_pos"].min()) if step.n_seqs else None)
+                                       int(step.host["first_pos"].min()) if step.n_seqs else None, step.n_tokens)
     ctx.group_tables = [by_name[f"tables{g}"] for g in range(n_groups)]
     ctx.group_slots = [by_name[f"slots{g}"] for g in range(n_groups)]
     ctx.n_tokens, ctx.n_seqs, ctx.n_logits = step.n_tokens, step.n_seqs, step.n_logits

@@ -96,7 +96,7 @@ class _DecodeGraph:
         lists = {f"tiles_multi_{t}": empty for t in ops.kernels.TILE_SIZES}
         lists.update({f"tiles_all_{t}": (every, S) for t in ops.kernels.TILE_SIZES})
         lists["decode_seqs"] = (None, S)        # every sequence brings one token, in order: no list needed
-        ctx.attention = ops.AttentionBatch(ctx.q_start, ctx.q_len, ctx.ctx_len, S, lists, ctx_bucket, ctx_bucket)
+        ctx.attention = ops.AttentionBatch(ctx.q_start, ctx.q_len, ctx.ctx_len, S, lists, ctx_bucket, ctx_bucket, rows=S)
         ctx.group_tables = [view(f"tables{g}").view(S, self.max_blocks[g]) for g in range(G)]
         ctx.group_slots = [view(f"slots{g}") for g in range(G)]
         ctx.n_tokens = ctx.n_seqs = ctx.n_logits = S

@@ -828,17 +828,18 @@ class AttentionBatch:
     """The device-side description of a step's sequences that `attention` reads."""
 
     def __init__(self, q_start, q_len, ctx_len, n_seqs: int, lists: dict, max_decode_ctx: int, max_ctx: int,
-                 mean_walk: int = 0, max_tile_ctx: int | None = None, one_query_keys: int = 0, first_query: int | None = None):
+                 mean_walk: int = 0, max_tile_ctx: int | None = None, one_query_keys: int = 0, first_query: int | None = None,
+                 rows: int | None = None):
         """`lists`: name -> (device int32 tensor, number of entries), names as in `attention_lists`;
         `max_decode_ctx`, `max_ctx`: the longest context among one-query sequences, and among all;
         `mean_walk`: the mean number of keys that a tile of queries walks, see `mean_tile_walk` (a hint for
         how the kernels share out the work; unknown: 0); `max_tile_ctx`: the longest context among sequences with several
         queries (a hint as well; by default the longest of all); `one_query_keys`: the sum of the one-query sequences'
         contexts (a hint as well; unknown: 0); `first_query`: the lowest position that any query stands at (None: unknown;
-        `attention_shared` asks for it)."""
+        `attention_shared` asks for it); `rows`: one behind the last query's row (None: unknown; likewise)."""
         self.q_start, self.q_len, self.ctx_len, self.n_seqs = q_start, q_len, ctx_len, n_seqs
         self.lists, self.max_decode_ctx, self.max_ctx = lists, max_decode_ctx, max_ctx
-        self.mean_walk, self.one_query_keys, self.first_query = mean_walk, one_query_keys, first_query
+        self.mean_walk, self.one_query_keys, self.first_query, self.rows = mean_walk, one_query_keys, first_query, rows
         self.max_tile_ctx = max_ctx if max_tile_ctx is None else max_tile_ctx
 
     @classmethod
@@ -852,7 +853,8 @@ class AttentionBatch:
         return cls(to(starts), to(q_lens), to(ctx_lens), len(q_lens), lists, max(decode_ctx, default=0),
                    max((int(c) for c in ctx_lens), default=0),
                    mean_tile_walk(q_lens, ctx_lens), max((int(c) for c, q in zip(ctx_lens, q_lens) if q > 1), default=0),
-                   sum(int(c) for c in decode_ctx), min((int(c) - int(q) for c, q in zip(ctx_lens, q_lens) if q > 0), default=None))
+                   sum(int(c) for c in decode_ctx), min((int(c) - int(q) for c, q in zip(ctx_lens, q_lens) if q > 0), default=None),
+                   sum(int(q) for q in q_lens))
 
 
 def attention_plan(dtype: torch.dtype, hd: int, page_size: int, nq: int, nkv: int, kind: int = 0) -> tuple[int, bool]:
@@ -997,7 +999,8 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     """Causal attention, as `attention` without a window, of a batch whose sequences all begin with the same `prefix` tokens: their keys
     and values are read once for all rows, and each sequence's own keys, from position `prefix` on, by its own queries.
 
-    Every query stands at position `prefix` or later (`batch.first_query` says so; a call that does not is refused).  The shared keys are
+    Every query stands at position `prefix` or later (`batch.first_query` says so; a call that does not is refused), and every
+    query's row is one of `out`'s (`batch.rows` likewise).  The shared keys are
     read through `prefix_table` (int32, the pages of tokens 0 .. prefix - 1), by default the first sequence's row of `block_tables`; a
     prefix that ends inside a page may have a copy of its end in each sequence's own page.  Any number of queries a sequence, any page
     size, head sizes up to 256.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new one); calls
@@ -1011,6 +1014,8 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
         softcap = 0.0
     if nkv <= 0 or nq <= 0 or nq % nkv or not 0 < hd <= MAX_SHARED_HEAD_DIM:
         raise KernelError(f"attention_shared: {nq} query heads of {hd} in {nkv} groups: heads of 1..{MAX_SHARED_HEAD_DIM} that divide into the groups expected")
+    if batch.rows is None or batch.rows > out.shape[0]:
+        raise KernelError(f"attention_shared: queries in {'an unknown number of' if batch.rows is None else batch.rows} rows do not fit the {out.shape[0]} rows of out")
     tiles, n_tiles = batch.lists["tiles_all_16"]
     stream = _here("attention_shared", q, k_pool, v_pool, block_tables, out, sinks, prefix_table, batch.q_start, batch.q_len, batch.ctx_len,
           tiles if n_tiles else None)
