@@ -317,8 +317,9 @@ def step_arrays(entries: list[StepEntry], cache, table_tokens: int | None = None
 
 def context_from(step: StepArrays, dev: list, n_groups: int, workspace: Workspace, act_dtype, attention_kind: int = 0,
                  max_decode_ctx: int | None = None, max_ctx: int | None = None, max_tile_ctx: int | None = None,
-                 mean_walk: int | None = None) -> StepContext:
-    """The step's context over the device copies `dev` of `step.arrays` (same order)."""
+                 mean_walk: int | None = None, recorded: bool = False) -> StepContext:
+    """The step's context over the device copies `dev` of `step.arrays` (same order).  `recorded`: later steps of the same shape run from it
+    too, so that it knows no values of this one: nothing on the host, no lowest position."""
     ctx = StepContext(workspace, act_dtype, attention_kind)
     by_name = dict(zip(step.names, dev))
     ctx.token_ids, ctx.positions, ctx.q_start = by_name["token_ids"], by_name["positions"], by_name["q_start"]
@@ -331,12 +332,12 @@ def context_from(step: StepArrays, dev: list, n_groups: int, workspace: Workspac
                                        step.max_ctx if max_ctx is None else max_ctx,
                                        step.mean_walk if mean_walk is None else mean_walk,
                                        step.max_tile_ctx if max_tile_ctx is None else max_tile_ctx, step.one_query_keys,
-                                       int(step.host["first_pos"].min()) if step.n_seqs else None, step.n_tokens)
+                                       int(step.host["first_pos"].min()) if step.n_seqs and not recorded else None, step.n_tokens)
     ctx.group_tables = [by_name[f"tables{g}"] for g in range(n_groups)]
     ctx.group_slots = [by_name[f"slots{g}"] for g in range(n_groups)]
     ctx.n_tokens, ctx.n_seqs, ctx.n_logits = step.n_tokens, step.n_seqs, step.n_logits
     ctx.max_q_len = step.max_q_len
-    ctx.host = step.host
+    ctx.host = {} if recorded else step.host
     return ctx
 
 

@@ -230,8 +230,8 @@ class _PortionGraph:
         longest = math.isqrt(first.max_tile_ctx * ctx_bucket)
         self.ctx = context_from(first, views, len(cache.groups), OwnedNames(workspace, ("logits",), runner.device),
                                 runner.dtype, runner.attention_kind, max_decode_ctx=ctx_bucket, max_ctx=ctx_bucket,
-                                max_tile_ctx=longest, mean_walk=first.mean_walk * longest // max(1, first.max_tile_ctx))
-        self.ctx.host = {}
+                                max_tile_ctx=longest, mean_walk=first.mean_walk * longest // max(1, first.max_tile_ctx),
+                                recorded=True)
         self.copied = None
         self.graph = None
         self.logits = None

@@ -1000,7 +1000,8 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     and values are read once for all rows, and each sequence's own keys, from position `prefix` on, by its own queries.
 
     Every query stands at position `prefix` or later (`batch.first_query` says so; a call that does not is refused), and every
-    query's row is one of `out`'s (`batch.rows` likewise).  The shared keys are
+    query's row is one of `out`'s (`batch.rows` likewise).  A recorded call holds for replays of which that is true as well and whose contexts are
+    no longer than `batch.max_ctx`; the engine's own recorded steps do not know where later queries stand, and there the call is refused.  The shared keys are
     read through `prefix_table` (int32, the pages of tokens 0 .. prefix - 1), by default the first sequence's row of `block_tables`; a
     prefix that ends inside a page may have a copy of its end in each sequence's own page.  Any number of queries a sequence, any page
     size, head sizes up to 256.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new one); calls
@@ -1017,6 +1018,8 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     if batch.rows is None or batch.rows > out.shape[0]:
         raise KernelError(f"attention_shared: queries in {'an unknown number of' if batch.rows is None else batch.rows} rows do not fit the {out.shape[0]} rows of out")
     tiles, n_tiles = batch.lists["tiles_all_16"]
+    if n_tiles and (prefix < 0 or batch.first_query is None or batch.first_query < prefix):
+        raise KernelError(f"attention_shared: a query at position {batch.first_query} does not stand behind a prefix of {prefix} tokens")
     stream = _here("attention_shared", q, k_pool, v_pool, block_tables, out, sinks, prefix_table, batch.q_start, batch.q_len, batch.ctx_len,
           tiles if n_tiles else None)
     if q.dim() != 2 or out.dim() != 2 or out.shape[1] != nq * hd or q.shape[0] < out.shape[0] or q.dtype != out.dtype \
@@ -1036,8 +1039,6 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
         if t.dtype != torch.int32 or t.numel() < n:
             raise KernelError(f"attention_shared: {what} must be {n} int32 values")
     max_ctx = int(batch.max_ctx)
-    if prefix < 0 or batch.first_query is None or batch.first_query < prefix:
-        raise KernelError(f"attention_shared: a query at position {batch.first_query} does not stand behind a prefix of {prefix} tokens")
     if max_ctx > block_tables.shape[1] * page_size:
         raise KernelError(f"attention_shared: a context of {max_ctx} tokens is longer than its block table ({block_tables.shape[1]} pages of {page_size})")
     if prefix_table is None:

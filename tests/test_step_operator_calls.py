@@ -25,3 +25,35 @@ def test_queries_that_out_has_no_rows_for():
     with pytest.raises(ops.KernelError, match="unknown number of rows"):
         shared(unknown, 2)
     assert ops.AttentionBatch.build([0], [7], "cpu").rows == 0
+
+
+def two_entries():
+    """Five tokens from position 0 and three from position 6, and the cache they lie in."""
+    from sprout_lm_amd.cache import CacheManager, PagedKVSpec
+    from sprout_lm_amd.engine.batch import StepEntry
+    cache = CacheManager([PagedKVSpec(1, 16)], block_size=4, num_blocks=8, max_sequences=3)
+    a, b = cache.create(), cache.create()
+    assert cache.reserve(a, 5) and cache.reserve(b, 9)
+    cache.commit(b, 6)
+    return cache, [StepEntry(a, [1, 2, 3, 4, 5], [4]), StepEntry(b, [7, 8, 9], [])]
+
+
+def context(step, cache, **options):
+    from sprout_lm_amd.engine.batch import Workspace, context_from
+    return context_from(step, [torch.from_numpy(a) for a in step.arrays], len(cache.groups), Workspace("cpu"), torch.float32, **options)
+
+
+def test_a_recorded_step_does_not_know_where_later_queries_stand(monkeypatch):
+    """The step that is recorded stands behind position 6, one that is replayed may stand before it."""
+    from sprout_lm_amd.engine import graphs
+    from sprout_lm_amd.engine.batch import Workspace, step_arrays
+    cache, entries = two_entries()
+    step = step_arrays(entries[1:], cache)
+    assert context(step, cache).attention.first_query == 6 and context(step, cache).attention.rows == 3
+    zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *size, pin_memory=False, **kw: zeros(*size, **kw))      # (without a GPU there is no pinned memory)
+    runner = type("Runner", (), dict(cache=cache, device="cpu", dtype=torch.float32, attention_kind=0))()
+    recorded = graphs._PortionGraph(runner, step, 16, Workspace("cpu")).ctx
+    assert recorded.host == {} and recorded.attention.first_query is None and recorded.attention.rows == 3
+    with pytest.raises(ops.KernelError, match="None does not stand behind"):
+        shared(recorded.attention, 3, prefix=6)
