@@ -315,6 +315,12 @@ def step_arrays(entries: list[StepEntry], cache, table_tokens: int | None = None
                       ops.mean_tile_walk(q_lens, ctx_len), sum(decode_ctx), host)
 
 
+def first_query(host: dict) -> int | None:
+    """The lowest position that a step's queries stand at (None: it has no query), from its arrays on the host."""
+    positions = host["positions"]
+    return int(positions.min()) if positions.size else None
+
+
 def context_from(step: StepArrays, dev: list, n_groups: int, workspace: Workspace, act_dtype, attention_kind: int = 0,
                  max_decode_ctx: int | None = None, max_ctx: int | None = None, max_tile_ctx: int | None = None,
                  mean_walk: int | None = None, recorded: bool = False) -> StepContext:
@@ -332,7 +338,7 @@ def context_from(step: StepArrays, dev: list, n_groups: int, workspace: Workspac
                                        step.max_ctx if max_ctx is None else max_ctx,
                                        step.mean_walk if mean_walk is None else mean_walk,
                                        step.max_tile_ctx if max_tile_ctx is None else max_tile_ctx, step.one_query_keys,
-                                       int(step.host["first_pos"].min()) if step.n_seqs and not recorded else None, step.n_tokens)
+                                       None if recorded else lambda: first_query(step.host), step.n_tokens)
     ctx.group_tables = [by_name[f"tables{g}"] for g in range(n_groups)]
     ctx.group_slots = [by_name[f"slots{g}"] for g in range(n_groups)]
     ctx.n_tokens, ctx.n_seqs, ctx.n_logits = step.n_tokens, step.n_seqs, step.n_logits

@@ -828,19 +828,24 @@ class AttentionBatch:
     """The device-side description of a step's sequences that `attention` reads."""
 
     def __init__(self, q_start, q_len, ctx_len, n_seqs: int, lists: dict, max_decode_ctx: int, max_ctx: int,
-                 mean_walk: int = 0, max_tile_ctx: int | None = None, one_query_keys: int = 0, first_query: int | None = None,
-                 rows: int | None = None):
+                 mean_walk: int = 0, max_tile_ctx: int | None = None, one_query_keys: int = 0, first_query=None, rows: int | None = None):
         """`lists`: name -> (device int32 tensor, number of entries), names as in `attention_lists`;
         `max_decode_ctx`, `max_ctx`: the longest context among one-query sequences, and among all;
         `mean_walk`: the mean number of keys that a tile of queries walks, see `mean_tile_walk` (a hint for
         how the kernels share out the work; unknown: 0); `max_tile_ctx`: the longest context among sequences with several
         queries (a hint as well; by default the longest of all); `one_query_keys`: the sum of the one-query sequences'
-        contexts (a hint as well; unknown: 0); `first_query`: the lowest position that any query stands at (None: unknown;
-        `attention_shared` asks for it); `rows`: one behind the last query's row (None: unknown; likewise)."""
+        contexts (a hint as well; unknown: 0); `first_query`: the lowest position that any query stands at, or a function
+        that finds it (None: unknown; `attention_shared` asks for it); `rows`: one behind the last query's row (None: unknown; likewise)."""
         self.q_start, self.q_len, self.ctx_len, self.n_seqs = q_start, q_len, ctx_len, n_seqs
         self.lists, self.max_decode_ctx, self.max_ctx = lists, max_decode_ctx, max_ctx
-        self.mean_walk, self.one_query_keys, self.first_query, self.rows = mean_walk, one_query_keys, first_query, rows
+        self.mean_walk, self.one_query_keys, self._first_query, self.rows = mean_walk, one_query_keys, first_query, rows
         self.max_tile_ctx = max_ctx if max_tile_ctx is None else max_tile_ctx
+
+    @property
+    def first_query(self) -> int | None:
+        if callable(self._first_query):
+            self._first_query = self._first_query()
+        return self._first_query
 
     @classmethod
     def build(cls, q_lens, ctx_lens, device) -> "AttentionBatch":

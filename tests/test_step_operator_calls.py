@@ -57,3 +57,23 @@ def test_a_recorded_step_does_not_know_where_later_queries_stand(monkeypatch):
     assert recorded.host == {} and recorded.attention.first_query is None and recorded.attention.rows == 3
     with pytest.raises(ops.KernelError, match="None does not stand behind"):
         shared(recorded.attention, 3, prefix=6)
+
+
+def test_the_lowest_position_is_looked_for_when_asked():
+    """A step's host work does not grow for a number that only `attention_shared` reads; entries without tokens have no query."""
+    from sprout_lm_amd.engine.batch import StepEntry, step_arrays
+    cache, entries = two_entries()
+    step = step_arrays(entries, cache)
+    looks = []
+
+    class Watched(dict):
+        def __getitem__(self, name):
+            looks.append(name)
+            return super().__getitem__(name)
+    step.host = Watched(step.host)
+    ctx = context(step, cache)
+    assert looks == []
+    assert ctx.attention.first_query == 0 and ctx.attention.first_query == 0 and len(looks) == 1
+    empty = StepEntry(cache.create(), [], [])
+    assert context(step_arrays([empty, entries[1]], cache), cache).attention.first_query == 6
+    assert context(step_arrays([empty], cache), cache).attention.first_query is None
