@@ -90,6 +90,7 @@ class Sampler:
         ops.verify_drafts(logits, tokens, ints[0], ints[1], uniform, ints[2], ints[3], self._workspace, temperature, draft_logits, draft_rows)
         both = torch.cat([tokens.reshape(-1), ints[2:].reshape(-1)]).tolist()      # 4 bytes a row cross the bus
         given, accepted, following = both[:rows], both[rows:rows + n], both[rows + n:]
-        if any(t < 0 for t in following):
+        answers = [given[start + 1:start + 1 + held] + [token] for start, held, token in zip(starts.tolist(), accepted, following)]
+        if any(t < 0 or t >= self.vocab_size for answer in answers for t in answer):      # (as `sample`: a padded head's rows are longer than the vocabulary)
             raise NonFiniteLogits("Non-finite logits: the model produced NaN or infinity.")
-        return [given[start + 1:start + 1 + held] + [token] for start, held, token in zip(starts.tolist(), accepted, following)]
+        return answers

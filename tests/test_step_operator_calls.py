@@ -77,3 +77,19 @@ def test_the_lowest_position_is_looked_for_when_asked():
     empty = StepEntry(cache.create(), [], [])
     assert context(step_arrays([empty, entries[1]], cache), cache).attention.first_query == 6
     assert context(step_arrays([empty], cache), cache).attention.first_query is None
+
+
+def test_the_sampler_gives_no_token_outside_its_vocabulary(monkeypatch):
+    """Rows longer than the vocabulary (a padded head): an id behind it is refused as `Sampler.sample` does, drawn or kept as a draft."""
+    from sprout_lm_amd.sampling import NonFiniteLogits, Sampler, SamplingParams
+    sampler, tokens = Sampler(torch.device("cpu"), 5), torch.tensor([1, 6, 2], dtype=torch.int32)
+
+    def verify(held, following):
+        def answer(logits, tokens, starts, lens, uniform, accepted, next_token, *rest):
+            accepted[:], next_token[:] = held, following
+        monkeypatch.setattr(ops, "verify_drafts", answer)
+        return sampler.verify(torch.zeros(3, 8), tokens, [3], [SamplingParams()], [0])
+    assert verify(0, 4) == [[4]]
+    for held, following in ((0, 5), (0, -1), (1, 3), (2, 3)):      # drawn: 5; refused by the kernel; the draft 6 kept
+        with pytest.raises(NonFiniteLogits):
+            verify(held, following)
