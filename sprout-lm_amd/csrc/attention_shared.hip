@@ -655,7 +655,8 @@ extern "C" int sp_attention_shared(void* stream, int dtype, const void* q, int q
   while ((1 << a.page_shift) < page_size && a.page_shift < 30) ++a.page_shift;
   const bool runs = hd % epc == 0 && page_size >= 16 && (1 << a.page_shift) == page_size && page_size <= 4096 && q_stride % epc == 0 && bases % 16 == 0;
   // blocks for the rows that an entry has on average (four rows a block); those of longer entries are walked in turns
-  const dim3 join_grid(n_tiles, ((tokens + n_tiles - 1) / n_tiles * nq + 3) / 4);
+  const int64_t in_entry = (tokens + n_tiles - 1) / n_tiles < kSharedTile ? (tokens + n_tiles - 1) / n_tiles : kSharedTile, of_four = (in_entry * nq + 3) / 4;
+  const dim3 join_grid(n_tiles, of_four < 16383 ? of_four : 16383);      // (times four below 65,536, the most along y)
   hipStream_t s = (hipStream_t)stream;
   return dtype == kF32 ? launch_shared_of<float>(s, a, int(blocks), held, runs, join_grid, out)
                        : launch_shared_of<bf16_t>(s, a, int(blocks), held, runs, join_grid, out);

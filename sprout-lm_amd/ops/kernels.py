@@ -1050,7 +1050,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
         prefix_table = block_tables      # the first row of it
     elif prefix_table.dtype != torch.int32 or prefix_table.numel() * page_size < prefix:
         raise KernelError(f"attention_shared: a prefix of {prefix} tokens is longer than its table ({prefix_table.numel()} pages of {page_size})")
-    T = out.shape[0]
+    T = batch.rows      # (rows of out behind them are no work and no workspace)
     if n_tiles > T:
         raise KernelError(f"attention_shared: {n_tiles} tiles of queries for {T} rows")
     need = _shared_workspace_floats(code, hd, nq, nkv, T, n_tiles, prefix, max_ctx)
