@@ -532,6 +532,9 @@ int keys_of_stage(int dtype, int held) {
   return bytes <= 128 ? 128 : bytes <= 256 ? 64 : 32;
 }
 
+// Rows of heads, numbers of a token and keys, with a part's or a block's more, are counted in 32 bits.
+bool shared_fits(int hd, int nq, int tokens, int max_ctx) { return int64_t(tokens) * nq <= 1 << 30 && int64_t(nq) * hd <= 1 << 30 && max_ctx <= 1 << 30; }
+
 struct SharedPlan { int prefix_splits, prefix_keys, row_blocks, block_rows, own_splits, own_keys, own_rows; };
 
 // How the work is cut: the shared keys of a block of rows into the number of parts with the least estimated time in microseconds.  A
@@ -607,7 +610,8 @@ template <typename E> int launch_shared_of(hipStream_t s, const SharedArgs& a, i
 using namespace sprout;
 
 extern "C" int64_t sp_attention_shared_workspace_floats(int dtype, int hd, int nq, int nkv, int tokens, int n_tiles, int prefix, int max_ctx) {
-  if (hd <= 0 || hd > 256 || nkv <= 0 || nq <= 0 || nq % nkv || tokens <= 0 || n_tiles <= 0 || n_tiles > tokens || prefix < 0 || max_ctx <= prefix) return 0;
+  if (hd <= 0 || hd > 256 || nkv <= 0 || nq <= 0 || nq % nkv || tokens <= 0 || n_tiles <= 0 || n_tiles > tokens || prefix < 0 || max_ctx <= prefix ||
+      !shared_fits(hd, nq, tokens, max_ctx)) return 0;
   const SharedPlan p = shared_plan(dtype, hd, nq, nkv, tokens, n_tiles, prefix, max_ctx - prefix);
   return (int64_t(p.prefix_splits) + p.own_splits) * tokens * nq * (held_dims(hd) + 2);
 }
@@ -625,6 +629,7 @@ extern "C" int sp_attention_shared(void* stream, int dtype, const void* q, int q
   if (n_tiles == 0) return 0;
   SP_REQUIRE(q && k_pool && v_pool && block_tables && q_start && q_len && ctx_len && tiles && out && (prefix_table || prefix == 0),
              "sp_attention_shared: null operand");
+  SP_REQUIRE(shared_fits(hd, nq, tokens, max_ctx), "sp_attention_shared: %d rows of %d heads of %d with contexts of up to %d are more than indexes hold", tokens, nq, hd, max_ctx);
   SP_REQUIRE(q_stride >= nq * hd, "sp_attention_shared: q row stride %d is smaller than %d", q_stride, nq * hd);
   SP_REQUIRE(prefix >= 0 && max_ctx > prefix && int64_t(max_ctx) <= int64_t(max_blocks) * page_size,
              "sp_attention_shared: a prefix of %d and contexts of up to %d do not fit %d pages of %d", prefix, max_ctx, max_blocks, page_size);
@@ -636,7 +641,7 @@ extern "C" int sp_attention_shared(void* stream, int dtype, const void* q, int q
              (long long)workspace_floats, (long long)need);
   const int64_t rows = int64_t(tokens) * nq, parts = int64_t(p.prefix_splits) + p.own_splits;
   const int64_t blocks = (int64_t(p.prefix_splits) * nkv + 7) / 8 * 8 * p.row_blocks + int64_t(p.own_splits) * n_tiles * p.own_rows * nkv;
-  SP_REQUIRE(blocks < (int64_t(1) << 31), "sp_attention_shared: too many blocks");
+  SP_REQUIRE(blocks < 1 << 24, "sp_attention_shared: %lld blocks are more than a launch takes", (long long)blocks);      // less than 2^32 threads
   SharedArgs a;
   a.q = q; a.k_pool = k_pool; a.v_pool = v_pool;
   a.block_tables = block_tables; a.prefix_table = prefix_table; a.q_start = q_start; a.q_len = q_len; a.ctx_len = ctx_len; a.tiles = tiles;

@@ -93,3 +93,18 @@ def test_the_sampler_gives_no_token_outside_its_vocabulary(monkeypatch):
     for held, following in ((0, 5), (0, -1), (1, 3), (2, 3)):      # drawn: 5; refused by the kernel; the draft 6 kept
         with pytest.raises(NonFiniteLogits):
             verify(held, following)
+
+
+def test_shared_attention_refuses_sizes_that_no_index_holds():
+    from sprout_lm_amd.ops.library import check
+    lib = ops.library()
+    #       stream dtype q stride k  v  tables max table prefix start len ctx tiles n max_ctx T ws floats out nq nkv hd page pages scale cap sinks
+    good = [None, 1, 16, 1 << 30, 16, 16, 16, 9, 16, 100, 16, 16, 16, 16, 2, 110, 2, 16, 1 << 60, 16, 4, 2, 64, 16, 9, 0.1, 0.0, None]
+    #       rows of heads; a token's numbers; keys; blocks of 128 rows of many groups
+    for changes, match in (({16: 1 << 29}, "indexes"), ({20: 1 << 25, 21: 1 << 25, 3: 2 ** 31 - 1}, "indexes"), ({7: 2 ** 27 - 1, 15: (1 << 30) + 1}, "indexes"),
+                           ({16: 1 << 17, 20: 1 << 13, 21: 1 << 13, 9: 64, 14: 1 << 17}, "launch")):
+        args = [changes.get(i, a) for i, a in enumerate(good)]
+        with pytest.raises(ops.KernelError, match=match):
+            check(lib.sp_attention_shared(*args))
+        floats = lib.sp_attention_shared_workspace_floats(args[1], args[22], args[20], args[21], args[16], args[14], args[9], args[15])
+        assert (floats == 0) == (match == "indexes")
