@@ -48,9 +48,13 @@ struct SharedArgs {
   float scale2, cap;                                           // scale in log2 units; with a cap (0: none) twice that over the cap
 };
 
-// cap tanh(x) in log2 units, of 2 x in log2 units: tanh x = 1 - 2 / (exp(2 x) + 1), off by 2^-23 of the cap like a rounded tanh itself.
+// cap tanh(x) in log2 units, of 2 x in log2 units: tanh x = 1 - 2 / (exp(2 x) + 1), off by some 2^-23; below 0.3, where that is more than
+// a few units of the result's last place and the cap may be far above the scores, the Taylor polynomial (5e-8 of the value).
 __device__ __forceinline__ float capped(float x2, float cap) {
-  return cap * kLog2E * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x2) + 1.f));
+  const float x = x2 * 0.34657359f, y = x * x;
+  const float near = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x2) + 1.f);
+  return cap * kLog2E * (fabsf(x) < 0.3f ? near : far);
 }
 
 template <typename E> struct Numbers;

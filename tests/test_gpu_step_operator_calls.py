@@ -25,3 +25,11 @@ def test_rows_behind_the_batch_are_no_work():
         got.append(case.run(workspace=workspace))
         case.check(got[-1], *case.definition())
     assert torch.equal(got[0], got[1]) and asked[0] == asked[1]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("cap", [0.5, 50.0, 1.0e6])
+def test_caps_below_and_far_above_the_scores(cap, dtype):
+    """A score far below its cap is the score but for its last places (10 times 2^-24 of it at most, less than what the product's own roundings are
+    allowed): scores reach some 8 here."""
+    shared.check(shared.Case(dtype, 4, 2, 64, 16, 140, [(1, 20), (3, 5)], seed=3), scores="capped", softcap=cap, definition={"cap": cap})
