@@ -637,7 +637,7 @@ extern "C" int sp_attention_shared(void* stream, int dtype, const void* q, int q
   SP_REQUIRE(q_stride >= nq * hd, "sp_attention_shared: q row stride %d is smaller than %d", q_stride, nq * hd);
   SP_REQUIRE(prefix >= 0 && max_ctx > prefix && int64_t(max_ctx) <= int64_t(max_blocks) * page_size,
              "sp_attention_shared: a prefix of %d and contexts of up to %d do not fit %d pages of %d", prefix, max_ctx, max_blocks, page_size);
-  SP_REQUIRE(softcap >= 0.f, "sp_attention_shared: negative cap");
+  SP_REQUIRE(softcap >= 0.f && softcap < INFINITY, "sp_attention_shared: a cap that is negative or not finite");
   const SharedPlan p = shared_plan(dtype, hd, nq, nkv, tokens, n_tiles, prefix, max_ctx - prefix);
   const int held = held_dims(hd);
   const int64_t need = sp_attention_shared_workspace_floats(dtype, hd, nq, nkv, tokens, n_tiles, prefix, max_ctx);

@@ -1014,8 +1014,8 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     to no sequence are left as they are."""
     code = _code(q, "q")
     if variant_code(SCORE_STAGES, scores, "score stage") == 1:
-        if not softcap > 0.0:
-            raise KernelError("attention_shared: capped scores need a positive cap")
+        if not 0.0 < softcap < float("inf"):
+            raise KernelError("attention_shared: capped scores need a positive cap that is finite")
     else:
         softcap = 0.0
     if nkv <= 0 or nq <= 0 or nq % nkv or not 0 < hd <= MAX_SHARED_HEAD_DIM:

@@ -108,3 +108,18 @@ def test_shared_attention_refuses_sizes_that_no_index_holds():
             check(lib.sp_attention_shared(*args))
         floats = lib.sp_attention_shared_workspace_floats(args[1], args[22], args[20], args[21], args[16], args[14], args[9], args[15])
         assert (floats == 0) == (match == "indexes")
+
+
+@pytest.mark.parametrize("cap", [float("inf"), float("nan"), 0.0, -1.0])
+def test_shared_attention_refuses_caps_that_are_no_number(cap):
+    """An infinite cap would make every score infinity times zero."""
+    from sprout_lm_amd.ops.library import check
+    batch = ops.AttentionBatch.build([1], [101], "cpu")
+    with pytest.raises(ops.KernelError, match="positive cap"):
+        shared(batch, 1, scores="capped", softcap=cap)
+    with pytest.raises(ops.KernelError, match="current GPU"):
+        shared(batch, 1, scores="scaled_dot", softcap=cap)      # (no cap is looked at)
+    args = [None, 1, 16, 256, 16, 16, 16, 9, 16, 100, 16, 16, 16, 16, 2, 110, 2, 16, 1 << 40, 16, 4, 2, 64, 16, 9, 0.1, cap, None]
+    if cap != 0.0:
+        with pytest.raises(ops.KernelError, match="cap"):
+            check(ops.library().sp_attention_shared(*args))
