@@ -654,8 +654,10 @@ def gemm_q4_workspace_floats(dtype: torch.dtype, T: int, N: int, K: int) -> int:
 
 def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False, workspace=None) -> None:
     """out = a @ w.T (+ bias) of a's dtype (float32 or bfloat16); with accumulate, out (float32) += a @ w.T (+ bias).  Made for few tokens: the
-    weights are read once for every 64.  bfloat16 numbers of `a` are multiplied by up to 31 and the excess taken off: beyond some 1e37, and
-    for an infinity, a token's row is NaN.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new
+    weights are read once for every 64.  bfloat16 numbers of `a` are multiplied by up to 31, and 24 times them is taken off, in float32: a number's share of
+    the error is 2^-24 of up to 40 times it, and where the magnitudes of a group's numbers sum to more than 2^122 (5e36) the sums may pass float32's
+    range and the token's results be infinite or NaN.  An infinity makes its token's row NaN, and so does a float32 number from 3.39e38 on, which
+    bfloat16, whose parts it is taken in, rounds to one.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new
     one, where the product needs any); calls that may run at the same time need one each."""
     stream = _here("gemm_q4", a, w.words, w.scales, out, bias)
     if a.dim() != 2 or a.shape[1] != w.cols or tuple(out.shape) != (a.shape[0], w.rows):
