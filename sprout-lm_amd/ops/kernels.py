@@ -656,7 +656,7 @@ def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor 
     """out = a @ w.T (+ bias) of a's dtype (float32 or bfloat16); with accumulate, out (float32) += a @ w.T (+ bias).  Made for few tokens: the
     weights are read once for every 64.  bfloat16 numbers of `a` are multiplied by up to 31, and 24 times them is taken off, in float32: a number's share of
     the error is 2^-24 of up to 40 times it, and where the magnitudes of a group's numbers sum to more than 2^122 (5e36) the sums may pass float32's
-    range and the token's results be infinite or NaN.  An infinity makes its token's row NaN, and so does a float32 number from 3.39e38 on, which
+    range and the token's results be infinite or NaN.  An infinity makes its token's row NaN, and so does a float32 number from 3.4e38 on, which
     bfloat16, whose parts it is taken in, rounds to one.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new
     one, where the product needs any); calls that may run at the same time need one each."""
     stream = _here("gemm_q4", a, w.words, w.scales, out, bias)
