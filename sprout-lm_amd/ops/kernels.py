@@ -600,6 +600,7 @@ class Q4Matrix:
 
     def __init__(self, rows: int, cols: int, group: int, words: torch.Tensor, scales: torch.Tensor):
         groups = _q4_sizes(rows, cols, group)
+        _code(scales, "4-bit weights' scales")
         if words.dtype != torch.int32 or words.numel() != library().sp_q4_words(rows, cols) or tuple(scales.shape) != (groups, (rows + 15) // 16 * 16):
             raise KernelError(f"4-bit weights [{rows}, {cols}] in groups of {group}: words {tuple(words.shape)} and scales {tuple(scales.shape)} do not fit")
         self.rows, self.cols, self.group, self.words, self.scales = rows, cols, group, words, scales

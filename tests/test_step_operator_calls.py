@@ -123,3 +123,12 @@ def test_shared_attention_refuses_caps_that_are_no_number(cap):
     if cap != 0.0:
         with pytest.raises(ops.KernelError, match="cap"):
             check(ops.library().sp_attention_shared(*args))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64, torch.int32])
+def test_4_bit_weights_refuse_scales_that_no_kernel_reads(dtype):
+    words = torch.zeros(2 * 2 * 256, dtype=torch.int32)
+    with pytest.raises(ops.KernelError, match="scales"):
+        ops.Q4Matrix(20, 130, 32, words, torch.zeros(5, 32).to(dtype))
+    for taken in (torch.float32, torch.bfloat16):
+        assert ops.Q4Matrix(20, 130, 32, words, torch.zeros(5, 32).to(taken)).group == 32
