@@ -16,11 +16,12 @@
 // of 16 bytes a dimension: 1 KB a read and 1 KB a load, whose lanes' addresses are one number a lane beside scalars.
 // Weights are rounded to bfloat16 for the product with the values (half a step each); the sum of the weights is of the unrounded ones.
 //
-// Heads of 128, bfloat16: 16 sequences of one query behind 32,000 keys (40 heads in 8 groups) 44.8 us, 3.3 TB/s; 64 of 1 to 5 queries behind
-// 8,192 keys and 64 to 1,024 own (28 heads in 4 groups) 54.5 us, 436 TFLOP/s.  Neither bytes nor products bound these: a stage of 64 keys by
-// 128 rows takes a CU 1.35 us, of which the matrix cores work 0.43 and the vector unit as long, one after the other in a wave, and two
-// blocks on a CU take more than twice as long as one; a sixth is the loads.  Small batches are bound by two launches and the trips from table to page to
-// product: four sequences behind 500 keys 8.8 + 4.1 us.
+// Heads of 128, bfloat16: 16 sequences of one query behind 32,000 keys (40 heads in 8 groups) 45.0 us, 3.3 TB/s; 64 of 1 to 5 queries behind
+// 8,192 keys and 64 to 1,024 own (28 heads in 4 groups) 55 us, 430 TFLOP/s.  Neither bytes nor products bound these: of the second's 46.6 us in
+// the first launch the matrix cores work 10 and the vector unit 11, and waves wait two fifths of their time.  A stage of 64 keys by 128 rows
+// takes 1.35 us for a block alone on the chip, 2.2 with one on every CU and 3.0 each with two, which is 1.36 times the work of one; but 352 blocks
+// of 16 stages leave 160 of the 256 CUs with one.  Small batches are bound by two launches and the trips from table to page to
+// product: four sequences behind 500 keys 9.9 + 3.9 us.
 #include <type_traits>
 
 #include "mfma.h"

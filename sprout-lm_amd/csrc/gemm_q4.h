@@ -17,9 +17,9 @@
 // share out K and a second launch joins them, in a fixed order.
 //
 // One token of bfloat16 by 37,888 x 3,584 in groups of 128: 15.8 us, 4.4 TB/s of weights and scales, near what a copy reaches.  64 tokens by
-// 55,296 x 5,120 in groups of 32: 85 us, 426 TFLOP/s, bound by the vector unit: a group of 32 along K of 16 rows and 16 tokens costs one
-// matrix instruction of 16 cycles, four float32 multiply-adds by the scale, 16 cycles, and of unpacking codes and scales 11 more (in groups
-// of 128: 66 us).  40 tokens of float32 by 3,584 x 18,944: 36.9 us, three products of bfloat16 each, 147 TFLOP/s of float32.
+// 55,296 x 5,120 in groups of 32: 85.7 us, 423 TFLOP/s, bound by the vector unit, which works 37 us beside the matrix cores' 22: a group of 32 along K of
+// 16 rows and 16 tokens costs one matrix instruction of 16 cycles, four float32 multiply-adds by the scale, 16 cycles, and of unpacking codes and
+// scales 11 more (in groups of 128: 66 us); 432 blocks are two on 176 CUs and one on 80.  40 tokens of float32 by 3,584 x 18,944: 36.9 us, three products of bfloat16 each, 147 TFLOP/s of float32.
 #pragma once
 #include "mfma.h"
 #include "sprout_hip.h"

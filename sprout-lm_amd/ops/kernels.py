@@ -655,7 +655,7 @@ def gemm_q4_workspace_floats(dtype: torch.dtype, T: int, N: int, K: int) -> int:
 
 def gemm_q4(a: torch.Tensor, w: Q4Matrix, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False, workspace=None) -> None:
     """out = a @ w.T (+ bias) of a's dtype (float32 or bfloat16); with accumulate, out (float32) += a @ w.T (+ bias).  Made for few tokens: the
-    weights are read once for every 64.  bfloat16 numbers of `a` are multiplied by up to 31, and 24 times them is taken off, in float32: a number's share of
+    weights are read once for every 64, and up to there it is the faster one beside `gemm` with bfloat16 weights.  bfloat16 numbers of `a` are multiplied by up to 31, and 24 times them is taken off, in float32: a number's share of
     the error is 2^-24 of up to 40 times it, and where the magnitudes of a group's numbers sum to more than 2^122 (5e36) the sums may pass float32's
     range and the token's results be infinite or NaN.  An infinity makes its token's row NaN, and so does a float32 number from 3.4e38 on, which
     bfloat16, whose parts it is taken in, rounds to one.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new
@@ -1014,7 +1014,10 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     prefix that ends inside a page may have a copy of its end in each sequence's own page.  Any number of queries a sequence, any page
     size, head sizes up to 256.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new one); calls
     that may run at the same time need one each.  `scores`, `softcap`, `sinks`: as for `attention`.  Rows of `out` that belong
-    to no sequence are left as they are."""
+    to no sequence are left as they are.
+
+    Faster than `attention` where it need not read some 32,000 keys again (sequences times prefix, one query each), with several queries a
+    sequence from some 2,000 shared keys on; below that two launches cost more than the keys."""
     code = _code(q, "q")
     if variant_code(SCORE_STAGES, scores, "score stage") == 1:
         if not 0.0 < softcap < float("inf"):
