@@ -1,19 +1,12 @@
 """Loads into LDS are written as assembly, whose waits the compiler does not count.  A load may read a scalar register five wait states after a
 vector instruction wrote it; the built library's kernels are walked along all their branches for loads that come sooner."""
-import os
 import re
-import shutil
-import struct
-import subprocess
-from concurrent.futures import ThreadPoolExecutor
 
-import pytest
+from tests.assembly_helpers import instructions, kernels_with, listing, wait_states
 
 WAIT_STATES = 5
 LOADS = ("global_", "buffer_", "flat_", "scratch_")
-NO_NEXT = ("s_branch", "s_endpgm", "s_setpc_b64")
 SCALARS = re.compile(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b|\b(vcc)")
-LINE = re.compile(r"\t(\S+)\s*(.*?)\s*// ([0-9A-F]+):.*?(?:<[^>+]*(?:\+0x([0-9a-f]+))?>)?$")
 
 
 def scalars(operand):
@@ -36,23 +29,13 @@ def written_by_vector(name, operands):
 
 def too_early(lines):
     """(vector instruction, load) of every load that reads a scalar register too soon, and how many loads into LDS there are."""
-    code, place = [], {}
-    for line in lines:
-        found = LINE.match(line)
-        if found:
-            name, operands, address, target = found.groups()
-            jump = int(target or "0", 16) if name == "s_branch" or name.startswith("s_cbranch") else None
-            place[int(address, 16)] = len(code)
-            code.append((name, operands, jump))
-    start = min(place) if place else 0
+    code, after = instructions(lines)
     before = [[] for _ in code]
-    for i, (name, _, jump) in enumerate(code):
-        if i + 1 < len(code) and name not in NO_NEXT:
-            before[i + 1].append(i)
-        if jump is not None:
-            before[place[start + jump]].append(i)
-    writes, bad = [written_by_vector(name, operands) for name, operands, _ in code], []
-    for i, (name, operands, _) in enumerate(code):
+    for i, places in enumerate(after):
+        for j in places:
+            before[j].append(i)
+    writes, bad = [written_by_vector(*c) for c in code], []
+    for i, (name, operands) in enumerate(code):
         reads = scalars(operands) if name.startswith(LOADS) else set()
         todo, least = [(j, 0) for j in before[i]] if reads else [], {}
         while todo:
@@ -61,30 +44,13 @@ def too_early(lines):
                 continue
             least[j] = waited
             if writes[j] & reads:
-                bad.append((" ".join(code[j][:2]), " ".join(code[i][:2])))
+                bad.append((" ".join(code[j]), " ".join(code[i])))
                 continue
-            states = int(code[j][1].split()[0], 0) + 1 if code[j][0] == "s_nop" else 1
-            todo += [(k, waited + states) for k in before[j]]
-    return bad, sum("load_lds" in name for name, _, _ in code)
-
-
-def kernels(text):
-    name, lines = None, []
-    for line in text.split("\n"):
-        head = re.match(r"(?:[0-9a-f]+ )?<(.+)>:$", line)
-        if head:
-            if name:
-                yield name, lines
-            name, lines = head.group(1), []
-        else:
-            lines.append(line)
-    if name:
-        yield name, lines
+            todo += [(k, waited + wait_states(*code[j])) for k in before[j]]
+    return bad, sum("load_lds" in name for name, _ in code)
 
 
 def test_the_walk_finds_what_it_looks_for():
-    def listing(*code):
-        return [f"\t{c} // {4 * i:012X}: 00000000" + (f" <k+0x{to:x}>" if to else "") for i, (c, to) in enumerate(code)]
     lane, load = ("v_readlane_b32 s5, v2, 3", 0), ("global_load_lds_dwordx4 v1, s[4:5]", 0)
     moves, more = ("s_mov_b32 m0, s9", 0), lambda n: (f"s_nop {n}", 0)
     assert too_early(listing(lane, moves, more(0), load)) == ([(lane[0], load[0])], 1)
@@ -96,27 +62,7 @@ def test_the_walk_finds_what_it_looks_for():
 
 
 def test_no_load_reads_a_scalar_too_early(tmp_path):
-    from sprout_lm_amd.csrc.build import ensure_built
-    tools = [shutil.which(name, path=os.environ.get("PATH", "") + ":/opt/rocm/llvm/bin") for name in ("llvm-objcopy", "llvm-objdump")]
-    if not all(tools):
-        pytest.skip("llvm-objcopy and llvm-objdump are not here")
-    subprocess.run([tools[0], "--dump-section", f".hip_fatbin={tmp_path}/all", ensure_built(), f"{tmp_path}/copy"], check=True)
-    data, at, objects = (tmp_path / "all").read_bytes(), 0, []
-    while (at := data.find(b"__CLANG_OFFLOAD_BUNDLE__", at)) >= 0:      # one a source: number of entries, then offset, size and name of each
-        entry = at + 32
-        for _ in range(struct.unpack_from("<Q", data, at + 24)[0]):
-            offset, size, name = struct.unpack_from("<QQQ", data, entry)
-            if b"gfx950" in data[entry + 24:entry + 24 + name]:
-                objects.append(tmp_path / f"{len(objects)}.co")
-                objects[-1].write_bytes(data[at + offset:at + offset + size])
-            entry += 24 + name
-        at += 24
-
-    def walk(path):
-        text = subprocess.run([tools[1], "-d", str(path)], check=True, capture_output=True, text=True).stdout
-        return [(name, *too_early(lines)) for name, lines in kernels(text) if any("load_lds" in line for line in lines)] if "load_lds" in text else []
-    with ThreadPoolExecutor(8) as pool:
-        found = [kernel for of_source in pool.map(walk, objects) for kernel in of_source]
+    found = kernels_with("load_lds", too_early, tmp_path)
     for part in ("attention_shared_kernel", "attention_rows", "gemm_q4_staged_kernel", "gemm_pipe", "gemm_quad"):
-        assert any(part in name and loads for name, _, loads in found), part
-    assert [(name, bad[0], len(bad)) for name, bad, _ in found if bad] == []
+        assert any(part in name and loads for name, (_, loads) in found), part
+    assert [(name, bad[0], len(bad)) for name, (bad, _) in found if bad] == []
