@@ -466,7 +466,8 @@ int sp_head_mix(void* stream, int dtype, const void* o, const float* talk, int n
 // sp_attention: the keys before `prefix` are read once for all rows, through prefix_table (the numbers of the pages that hold them, the
 // prefix may end inside one), the keys from `prefix` up to a query's own through the sequence's row of block_tables.  Every query stands at
 // `prefix` or later.  tiles: (sequence, first query) of every tile of 16 queries of every sequence; max_ctx: the longest context; `tokens`:
-// rows of q and out; rows that belong to no sequence are left as they are.  head sizes up to 256; softcap 0: scores as they are;
+// rows of q and out, among them every query's; rows that belong to no sequence are left as they are.  head sizes up to 256; softcap 0: scores as they
+// are, otherwise a finite cap;
 // sinks (null: none): float32 [nq], a logit per head that joins the denominator.  A row that sees no key but by weights of zero is zeros.
 int64_t sp_attention_shared_workspace_floats(int dtype, int hd, int nq, int nkv, int tokens, int n_tiles, int prefix, int max_ctx);
 int sp_attention_shared(void* stream, int dtype, const void* q, int q_stride, const void* k_pool, const void* v_pool,
