@@ -1008,8 +1008,8 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
     and values are read once for all rows, and each sequence's own keys, from position `prefix` on, by its own queries.
 
     Every query stands at position `prefix` or later (`batch.first_query` says so; a call that does not is refused), and every
-    query's row is one of `out`'s (`batch.rows` likewise).  A recorded call holds for replays of which that is true as well and whose contexts are
-    no longer than `batch.max_ctx`; the engine's own recorded steps do not know where later queries stand, and there the call is refused.  The shared keys are
+    query's row is one of `out`'s (`batch.rows` likewise).  A recorded call holds for replays of which both are true as well, with the same list of
+    tiles and contexts no longer than `batch.max_ctx`; the engine's own recorded steps do not know where later queries stand, and there the call is refused.  The shared keys are
     read through `prefix_table` (int32, the pages of tokens 0 .. prefix - 1), by default the first sequence's row of `block_tables`; a
     prefix that ends inside a page may have a copy of its end in each sequence's own page.  Any number of queries a sequence, any page
     size, head sizes up to 256.  `workspace(n)` must return a float32 device tensor of at least n elements (default: a new one); calls
@@ -1056,7 +1056,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_pool: torch.Tensor, v_poo
         prefix_table = block_tables      # the first row of it
     elif prefix_table.dtype != torch.int32 or prefix_table.numel() * page_size < prefix:
         raise KernelError(f"attention_shared: a prefix of {prefix} tokens is longer than its table ({prefix_table.numel()} pages of {page_size})")
-    T = batch.rows      # (rows of out behind them are no work and no workspace)
+    T = out.shape[0]      # (not the batch's rows: a recorded call may be replayed with more of out's)
     if n_tiles > T:
         raise KernelError(f"attention_shared: {n_tiles} tiles of queries for {T} rows")
     need = _shared_workspace_floats(code, hd, nq, nkv, T, n_tiles, prefix, max_ctx)
